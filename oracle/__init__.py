@@ -453,3 +453,44 @@ def kld_threshold(hist, width, bins=2048, return_kl=False):
     t = lib().orc_kld_threshold(h.ctypes.data_as(C.c_void_p), C.c_float(width), bins,
                                 kl.ctypes.data_as(C.c_void_p))
     return (t, kl) if return_kl else t
+
+
+# ---- operators without a counterpart in the reference: from their definitions, in 64 bits, unrounded
+def activation64(x, kind):
+    """none, relu, silu, gelu (exact), gelu_tanh of a float64 array; relu keeps NaN."""
+    from math import erfc
+    x = np.asarray(x, np.float64)
+    with np.errstate(over="ignore", invalid="ignore"):
+        if kind == "relu":
+            return np.where(x < 0, 0.0, x)
+        if kind == "silu":
+            return x / (1.0 + np.exp(-x))
+        if kind == "gelu":
+            return x * 0.5 * np.vectorize(erfc, otypes=[np.float64])(-x / np.sqrt(2.0)) if x.size else x
+        if kind == "gelu_tanh":
+            return 0.5 * x * (1.0 + np.tanh(np.sqrt(2.0 / np.pi) * (x + 0.044715 * x ** 3)))
+    assert kind == "none", kind
+    return x
+
+
+def group_norm64(x, groups, gamma=None, beta=None, eps=1e-5, act="none"):
+    """Group norm of an NC... array with an affine per channel and an activation (layer norm: groups 1, rank 2)."""
+    x = np.asarray(x, np.float64)
+    n, c = x.shape[0], x.shape[1] if x.ndim > 1 else 1
+    t = x.reshape(n, groups, -1)
+    t = (t - t.mean(2, keepdims=True)) / np.sqrt(t.var(2, keepdims=True) + float(np.float32(eps)))
+    t = t.reshape(n, c, -1)
+    if gamma is not None:
+        t = t * np.asarray(gamma, np.float64)[None, :, None]
+    if beta is not None:
+        t = t + np.asarray(beta, np.float64)[None, :, None]
+    return activation64(t, act).reshape(x.shape)
+
+
+def linear64(x, w, bias=None, act="none", residual=None):
+    """act(x w^T + bias) + residual"""
+    y = np.asarray(x, np.float64) @ np.asarray(w, np.float64).T
+    if bias is not None:
+        y = y + np.asarray(bias, np.float64)
+    y = activation64(y, act)
+    return y if residual is None else y + np.asarray(residual, np.float64)

@@ -76,6 +76,13 @@ def run(text, weights, inputs, upto=None):
                                 stride=(_i(a, "sh", 1), _i(a, "sw", 1)), pad=(_i(a, "pt"), _i(a, "pl")),
                                 dilation=(_i(a, "dh", 1), _i(a, "dw", 1)), groups=_i(a, "g", 1),
                                 do_relu=bool(_i(a, "do_relu")))
+        elif t == "fully_connected" and ("activation" in a or (len(ins) > 7 and ins[7] != "-")):
+            act = "relu" if _i(a, "do_relu") else a.get("activation", "none")
+            out = O.linear64(X(0).reshape(X(0).shape[0], -1), W(1), W(2), act, X(7) if len(ins) > 7 and ins[7] != "-" else None)
+            out = O.bf16_round(out.astype(np.float32)) if op["dtype"] == "BF16" else out
+        elif t == "group_norm":
+            out = O.group_norm64(X(0), _i(a, "groups"), W(1), W(2), float(a.get("variance_epsilon", 1e-5)), a.get("activation", "none"))
+            out = O.bf16_round(out.astype(np.float32)) if op["dtype"] == "BF16" else out
         elif t == "fully_connected":
             x = X(0)
             if W(1).ndim >= 3:   # batched: one product per leading filter index (core/fullyconnected.cpp:59-88)

@@ -1,0 +1,158 @@
+"""group_norm and fully_connected with activation / residual, what needs no GPU: the checks of the arguments (compiled for the host)
+and the oracle's definitions against torch's."""
+import os
+import subprocess
+
+import numpy as np
+import pytest
+import torch
+
+import oracle as O
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+CHECKS = r"""
+#include "norm_linear.h"
+#include <iostream>
+using namespace tpucb;
+// stdin: weight lines "w name d0,d1,..", then op lines; the results of input ops are their operands. stdout: a line per other op.
+int main() {
+  std::map<std::string, HostWeight> weights;
+  std::map<std::string, DevTensor> tensors;
+  for (std::string line; std::getline(std::cin, line);) {
+    if (line.rfind("w ", 0) == 0) {
+      std::stringstream ss(line.substr(2));
+      std::string name, dims;
+      ss >> name >> dims;
+      HostWeight w;
+      size_t n = 1;
+      for (auto &d : split(dims, ',')) { w.shape.push_back(atoll(d.c_str())); n *= w.shape.back(); }
+      w.data.assign(n, 0.5f);
+      weights[name] = w;
+      continue;
+    }
+    const ParsedOp op = parse_line(line);
+    DevTensor t;
+    t.dtype = op.dtype == "INT8" ? 0 : (op.dtype == "BF16" ? 1 : 2);
+    int64_t d[4] = {1, 1, 1, 1};
+    for (size_t i = 0; i < op.shape.size(); ++i) d[i] = op.shape[i];
+    t.n = d[0]; t.c = d[1]; t.h = d[2]; t.w = t.wphys = d[3];
+    t.cp = round_up(t.c, t.dtype == 2 ? 4 : 16);
+    if (op.type == "input") { tensors[op.name] = t; continue; }
+    auto weight = [&](const std::string &nm) -> const HostWeight & {
+      TPUCB_CHECK(weights.count(nm), "weight '%s' was not registered", nm.c_str());
+      return weights[nm];
+    };
+    try {
+      if (op.type == "group_norm") {
+        const GroupNormSpec s = group_norm_spec(op, tensors.at(op.in[0]), t, weight);
+        std::cout << "ok groups=" << s.groups << " act=" << s.act << " eps=" << s.eps << " gamma0=" << s.gamma[0] << " gammas=" << s.gamma.size() << std::endl;
+      } else if (!linear_asked_for(op)) {
+        std::cout << "plain" << std::endl;
+      } else {
+        const DevTensor *res = names_operand(op, 7) ? &tensors.at(op.in[7]) : nullptr;
+        const LinearSpec s = linear_spec(op, tensors.at(op.in[0]), t, res, weight);
+        std::cout << "ok m=" << s.m << " n=" << s.n << " k=" << s.k_dev << " act=" << s.act << " bias0=" << s.bias[0] << std::endl;
+      }
+    } catch (const Error &e) {
+      std::cout << "refused: " << e.what() << std::endl;
+    }
+  }
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def checks(tmp_path_factory):
+    d = tmp_path_factory.mktemp("checks")
+    src, exe = d / "t.cpp", str(d / "t")
+    src.write_text(CHECKS)
+    subprocess.run(["g++", "-O1", "-std=c++17", "-I", os.path.join(ROOT, "tpu_compiler_b200", "csrc"), "-I", "/usr/local/cuda/include",
+                    str(src), "-o", exe], check=True)
+
+    def run(lines):
+        return subprocess.run([exe], input="\n".join(lines) + "\n", capture_output=True, text=True, check=True).stdout.splitlines()
+    return run
+
+
+NORM_IN = ["w g 48", "w b 48", "w short 47", "input name=x shape=2,48,5,3 dtype=BF16", "input name=q shape=2,48,5,3 dtype=INT8",
+           "input name=none shape=0,48 dtype=BF16"]
+
+
+@pytest.mark.parametrize("line,answer", [
+    ("group_norm name=y in=x,g,b shape=2,48,5,3 dtype=BF16 groups=4 activation=silu variance_epsilon=1e-6",
+     "ok groups=4 act=2 eps=1e-06 gamma0=0.5 gammas=48"),
+    ("group_norm name=y in=x,-,- shape=2,48,5,3 dtype=BF16 groups=48", "ok groups=48 act=0 eps=1e-05 gamma0=1 gammas=48"),
+    ("group_norm name=y in=x shape=2,48,5,3 dtype=BF16 groups=1 activation=gelu", "ok groups=1 act=3 eps=1e-05 gamma0=1 gammas=48"),
+    ("group_norm name=y in=x,g,b shape=2,48,5,3 dtype=BF16", "does not divide"),
+    ("group_norm name=y in=x,g,b shape=2,48,5,3 dtype=BF16 groups=5", "does not divide"),
+    ("group_norm name=y in=x,g,b shape=2,48,5,3 dtype=BF16 groups=-4", "does not divide"),
+    ("group_norm name=y in=x,g,b shape=2,48,5,3 dtype=FP32 groups=4", "one type"),
+    ("group_norm name=y in=q,g,b shape=2,48,5,3 dtype=INT8 groups=4", "BF16 and fp32 are implemented"),
+    ("group_norm name=y in=x,g,b shape=2,48,5,4 dtype=BF16 groups=4", "differ in shape"),
+    ("group_norm name=y in=x,g,b shape=2,48,5,3 dtype=BF16 groups=4 activation=mish", "is none of"),
+    ("group_norm name=y in=x,g,b shape=2,48,5,3 dtype=BF16 groups=4 variance_epsilon=0", "must be a positive"),
+    ("group_norm name=y in=x,g,b shape=2,48,5,3 dtype=BF16 groups=4 variance_epsilon=-1e-5", "must be a positive"),
+    ("group_norm name=y in=x,g,b shape=2,48,5,3 dtype=BF16 groups=4 variance_epsilon=nan", "must be a positive"),
+    ("group_norm name=y in=x,g,b shape=2,48,5,3 dtype=BF16 groups=4 variance_epsilon=1e-60", "must be a positive"),
+    ("group_norm name=y in=x,short,b shape=2,48,5,3 dtype=BF16 groups=4", "47 values, expected 48"),
+    ("group_norm name=y in=x,g,lost shape=2,48,5,3 dtype=BF16 groups=4", "was not registered"),
+    ("group_norm name=y in=none,-,- shape=0,48 dtype=BF16 groups=4", "empty tensor"),
+])
+def test_group_norm_arguments(checks, line, answer):
+    got, = checks(NORM_IN + [line])
+    assert answer in got and got.startswith("ok" if answer.startswith("ok") else "refused"), got
+
+
+LINEAR_IN = ["w f 20,48", "w img 20,720", "w batched 2,20,48", "w b 20", "w b19 19", "input name=x shape=3,48 dtype=BF16",
+             "input name=xi shape=3,48,5,3 dtype=BF16", "input name=x32 shape=3,40 dtype=FP32", "w f32 20,40", "input name=q shape=3,48 dtype=INT8",
+             "input name=r shape=3,20 dtype=BF16", "input name=rbad shape=4,20 dtype=BF16", "input name=r32 shape=3,20 dtype=FP32",
+             "input name=none shape=0,48 dtype=BF16", "input name=long shape=1,16,20000,20000 dtype=BF16"]
+
+
+@pytest.mark.parametrize("line,answer", [
+    ("fully_connected name=y in=x,f,b shape=3,20 dtype=BF16", "plain"),
+    ("fully_connected name=y in=x,f,b,-,-,-,-,- shape=3,20 dtype=BF16 do_relu=1", "plain"),
+    ("fully_connected name=y in=x,f,b shape=3,20 dtype=BF16 activation=none", "ok m=3 n=20 k=48 act=0 bias0=0.5"),
+    ("fully_connected name=y in=x,f shape=3,20 dtype=BF16 activation=gelu_tanh", "ok m=3 n=20 k=48 act=4 bias0=0"),
+    ("fully_connected name=y in=x,f,-,-,-,-,-,r shape=3,20 dtype=BF16 do_relu=1", "ok m=3 n=20 k=48 act=1 bias0=0"),
+    ("fully_connected name=y in=xi,img,b shape=3,20 dtype=BF16 activation=silu", "ok m=3 n=20 k=720 act=2 bias0=0.5"),
+    ("fully_connected name=y in=x32,f32,b,-,-,-,-,r32 shape=3,20 dtype=FP32", "ok m=3 n=20 k=40 act=0 bias0=0.5"),
+    ("fully_connected name=y in=x,f,b shape=3,20 dtype=BF16 activation=swish", "is none of"),
+    ("fully_connected name=y in=x,f,b shape=3,20 dtype=BF16 activation=relu do_relu=1", "exclude each other"),
+    ("fully_connected name=y in=q,f,b shape=3,20 dtype=INT8 activation=relu", "need a BF16 or fp32"),
+    ("fully_connected name=y in=x,f,b shape=3,20 dtype=FP32 activation=relu", "need a BF16 or fp32"),
+    ("fully_connected name=y in=x,batched,b shape=3,20 dtype=BF16 activation=relu", "batched"),
+    ("fully_connected name=y in=x,f,b shape=3,21 dtype=BF16 activation=relu", "filter has 960 values, expected n*k = 1008"),
+    ("fully_connected name=y in=x,f,b19 shape=3,20 dtype=BF16 activation=relu", "bias has 19 values"),
+    ("fully_connected name=y in=x,f,lost shape=3,20 dtype=BF16 activation=relu", "was not registered"),
+    ("fully_connected name=y in=x,f,b shape=2,20 dtype=BF16 activation=relu", r"output must be [m, n]"),
+    ("fully_connected name=y in=x,f,b shape=3,20,1,2 dtype=BF16 activation=relu", r"output must be [m, n]"),
+    ("fully_connected name=y in=x,f,b,-,-,-,-,rbad shape=3,20 dtype=BF16", "residual rbad must be"),
+    ("fully_connected name=y in=x,f,b,-,-,-,-,r32 shape=3,20 dtype=BF16", "residual r32 must be"),
+    ("fully_connected name=y in=none,f,b shape=0,20 dtype=BF16 activation=relu", "empty"),
+    ("fully_connected name=y in=long,f,b shape=1,20 dtype=BF16 activation=relu", "too long"),
+    ("fully_connected name=y in=x shape=3,20 dtype=BF16 activation=relu", "expects input, filter"),
+])
+def test_linear_arguments(checks, line, answer):
+    got, = checks(LINEAR_IN + [line])
+    assert answer in got and (got.startswith("refused") or answer.startswith(("ok", "plain"))), got
+
+
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "gelu_tanh"])
+def test_oracle_definitions_against_torch(act):
+    """2^-45: some hundred roundings of 2^-53 each."""
+    f = {"none": lambda v: v, "relu": torch.relu, "silu": torch.nn.functional.silu, "gelu": torch.nn.functional.gelu,
+         "gelu_tanh": lambda v: torch.nn.functional.gelu(v, approximate="tanh")}[act]
+    rng = np.random.default_rng(3)
+    x, g, b = rng.normal(1, 2, (2, 12, 5, 3)), rng.normal(1, 0.2, 12), rng.normal(0, 0.2, 12)
+    eps = float(np.float32(1e-3))
+    for groups in (1, 3, 12):
+        want = f(torch.nn.functional.group_norm(torch.tensor(x), groups, torch.tensor(g), torch.tensor(b), eps)).numpy()
+        assert np.abs(O.group_norm64(x, groups, g, b, 1e-3, act) - want).max() < 2 ** -45 * 16
+    rows = x.reshape(24, 15)
+    want = f(torch.nn.functional.layer_norm(torch.tensor(rows), (15,), None, None, eps)).numpy()
+    assert np.abs(O.group_norm64(rows, 1, None, None, 1e-3, act) - want).max() < 2 ** -45 * 16
+    w, bias, r = rng.normal(0, 1, (7, 15)), rng.normal(0, 1, 7), rng.normal(0, 1, (24, 7))
+    want = (f(torch.tensor(rows) @ torch.tensor(w).T + torch.tensor(bias)) + torch.tensor(r)).numpy()
+    assert np.abs(O.linear64(rows, w, bias, act, r) - want).max() < 2 ** -45 * 64

@@ -12,6 +12,8 @@
 #include "f32_kernels.cuh"
 #include "calib_kernels.cuh"
 #include "extra_kernels.cuh"
+#include "group_norm.cuh"
+#include "linear.cuh"
 #include "module_text.h"
 
 #include <algorithm>
@@ -1877,6 +1879,67 @@ private:
   size_t smem_ = 0;
 };
 
+// ------------------------------------------------- fully_connected with activation / residual
+// An inner product of BF16 or fp32 rows whose line names an activation (`activation=none|relu|silu|gelu|gelu_tanh`) or, as
+// operand 7 behind the quantisation operands, a residual tensor: y = act(x W^T + bias) + residual. No counterpart in the
+// reference, whose inner product ends in bias and ReLU (core/fullyconnected.cpp:44-91).
+class LinearOp : public OpKernel {
+public:
+  LinearOp(Interpreter &I, const ParsedOp &op, TensorPtr in, TensorPtr out) : in_(in), out_(out) {
+    if (names_operand(op, 7)) res_ = I.tensor(op.in[7]);
+    const LinearSpec s = linear_spec(op, *in, *out, res_.get(), [&](const std::string &nm) -> const HostWeight & { return I.weight(nm); });
+    act_ = s.act;
+    a_ = LinearArgs{};
+    a_.m = s.m; a_.k = s.k_dev; a_.n = s.n; a_.ldy = out->cp;
+    a_.x = in->dev;
+    a_.y = out->dev;
+    a_.res = res_ ? res_->dev : nullptr;
+    a_.bias = I.upload(s.bias);
+    // weights in the device's order of K, (y, x, c) with the input's channel pitch; rows of padded channels are zero
+    const size_t k = (size_t)in->c * s.hw;
+    auto packed = [&](auto zero, auto conv) {
+      std::vector<decltype(zero)> w((size_t)out->cp * s.k_dev, zero);
+      for (int j = 0; j < s.n; ++j) {
+        const float *src = s.filter->data.data() + (size_t)j * k;
+        auto *dst = w.data() + (size_t)j * s.k_dev;
+        for (int p = 0; p < s.hw; ++p)
+          for (int c = 0; c < in->c; ++c) dst[(size_t)p * in->cp + c] = conv(src[(size_t)c * s.hw + p]);
+      }
+      return (const void *)I.upload(w);
+    };
+    a_.w = out->dtype == DT_F32 ? packed(0.0f, [](float v) { return v; }) : packed((uint16_t)0, [](float v) { return f32_to_bf16_bits(v); });
+    alg_ops = 2.0 * s.m * k * s.n;
+    alg_bytes = (double)out->elsize() * ((double)s.m * k + (double)s.n * k + (double)s.m * s.n * (res_ ? 2 : 1)) + 4.0 * s.n;
+  }
+  void invoke(cudaStream_t s) override { launch_linear(a_, out_->dtype == DT_F32, act_, s); }
+  std::string form() const override { return "tiles=direct"; }
+
+private:
+  TensorPtr in_, out_, res_;
+  LinearArgs a_;
+  int act_ = ACT_NONE;
+};
+
+// ------------------------------------------------------------------------- group norm
+// group_norm (group_norm_spec): BF16 and fp32, rank 1 to 4, statistics per image over (h, w) and the c / groups channels of a
+// group; groups = 1 on [tokens, channels] is layer norm. No counterpart in the reference.
+class GroupNormOp : public OpKernel {
+public:
+  GroupNormOp(Interpreter &I, const ParsedOp &op, TensorPtr in, TensorPtr out) : in_(in), out_(out) {
+    const GroupNormSpec s = group_norm_spec(op, *in, *out, [&](const std::string &nm) -> const HostWeight & { return I.weight(nm); });
+    act_ = s.act;
+    a_ = GroupNormArgs{in->dev, out->dev, I.upload(s.gamma), I.upload(s.beta), in->n, in->h * in->w, in->c, in->cp, s.groups, in->c / s.groups, s.eps};
+    alg_ops = 8.0 * in->numel();
+    alg_bytes = 2.0 * in->numel() * in->elsize() + 8.0 * in->c;
+  }
+  void invoke(cudaStream_t s) override { launch_group_norm(a_, out_->dtype == DT_F32, act_, s); }
+
+private:
+  TensorPtr in_, out_;
+  GroupNormArgs a_;
+  int act_ = ACT_NONE;
+};
+
 // ====================================================================== Interpreter bodies
 
 // Who writes the remainder operand (x minus the upper 19 bits of x) of the fp32 tensors that TF32 x 3 convolutions read:
@@ -2039,7 +2102,7 @@ inline bool op_is_slot_safe(const std::string &t) {
   static const char *ok[] = {"input", "quant", "conv_2d", "deconv_2d", "fully_connected", "pool_max_2d", "pool_avg_2d",
                              "eltwise_add", "eltwise_mul", "eltwise_max", "eltwise_min", "concat", "upsample", "pixelshuffle",
                              "relu", "leaky_relu", "sigmoid", "mish", "exp", "tanh", "reciprocal", "scale", "batchnorm",
-                             "softmax", "reshape"};
+                             "softmax", "reshape", "group_norm"};
   for (const char *o : ok)
     if (t == o) return true;
   return false;
@@ -2134,6 +2197,8 @@ inline int Interpreter::add_op(const ParsedOp &op_in) {
       TPUCB_CHECK(cop.geti("pt") >= 0 && cop.geti("pl") >= 0, "deconv_2d %s: padding larger than the dilated filter extent",
                   op.name.c_str());
       k.reset(new Conv2DOp(*this, cop, opd(0), out));
+    } else if (op.type == "fully_connected" && linear_asked_for(op)) {
+      k.reset(new LinearOp(*this, op, opd(0), out));
     } else if (op.type == "fully_connected") {
       k.reset(new FullyConnectedOp(*this, op, opd(0), out));
     } else if (op.type == "pool_max_2d" || op.type == "pool_avg_2d") {
@@ -2180,6 +2245,8 @@ inline int Interpreter::add_op(const ParsedOp &op_in) {
       k.reset(new ScaleOp(*this, op, opd(0), out));
     } else if (op.type == "batchnorm") {
       k.reset(new BatchNormOp(*this, op, opd(0), out));
+    } else if (op.type == "group_norm") {
+      k.reset(new GroupNormOp(*this, op, opd(0), out));
     } else if (op.type == "softmax") {
       k.reset(new SoftmaxOp(*this, op, opd(0), out));
     } else {

@@ -1,0 +1,100 @@
+// What the module text says of a group_norm and of a fully_connected with activation or residual: arguments, checked before
+// anything is built. Host only.
+#pragma once
+#include "module_text.h"
+
+#include <cmath>
+#include <functional>
+
+namespace tpucb {
+
+enum Activation { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_GELU_TANH = 4 };
+
+inline int activation_from_string(const std::string &name, const std::string &op) {
+  static const char *names[] = {"none", "relu", "silu", "gelu", "gelu_tanh"};
+  for (int i = 0; i < 5; ++i)
+    if (name == names[i]) return i;
+  throw Error(strfmt("%s: activation '%s' is none of none, relu, silu, gelu, gelu_tanh", op.c_str(), name.c_str()));
+}
+
+using WeightOf = std::function<const HostWeight &(const std::string &)>;
+
+inline bool names_operand(const ParsedOp &op, size_t i) { return i < op.in.size() && op.in[i] != "-" && !op.in[i].empty(); }
+
+// group_norm: operands input, gamma, beta ("-": ones, zeros); attributes groups, variance_epsilon (1e-5), activation (none).
+struct GroupNormSpec {
+  int groups = 1, act = ACT_NONE;
+  float eps = 1e-5f;
+  std::vector<float> gamma, beta; // with the channel pitch, zero behind the channels
+};
+inline GroupNormSpec group_norm_spec(const ParsedOp &op, const DevTensor &in, const DevTensor &out, const WeightOf &weight) {
+  const char *nm = op.name.c_str();
+  TPUCB_CHECK(in.dtype == out.dtype && out.dtype != 0, "group_norm %s: BF16 and fp32 are implemented, input and result of one type", nm);
+  TPUCB_CHECK(in.n == out.n && in.c == out.c && in.h == out.h && in.w == out.w && in.cp == out.cp && !in.padded_rows() && !out.padded_rows(),
+              "group_norm %s: input and result differ in shape", nm);
+  TPUCB_CHECK(in.n > 0 && in.c > 0 && in.h > 0 && in.w > 0, "group_norm %s: empty tensor", nm);
+  GroupNormSpec s;
+  s.groups = op.geti("groups", 0);
+  TPUCB_CHECK(s.groups > 0 && in.c % s.groups == 0, "group_norm %s: groups = %d does not divide the %d channels", nm, s.groups, in.c);
+  s.eps = (float)op.getf("variance_epsilon", 1e-5);
+  TPUCB_CHECK(s.eps > 0.0f && std::isfinite(s.eps), "group_norm %s: variance_epsilon must be a positive fp32 number", nm);
+  s.act = activation_from_string(op.gets("activation", "none"), "group_norm " + op.name);
+  TPUCB_CHECK((double)in.h * in.w < 2147483648.0 && (double)in.n * s.groups < 2147483648.0, "group_norm %s: too many pixels or groups", nm);
+  auto affine = [&](size_t i, float absent) {
+    std::vector<float> v(in.cp, 0.0f);
+    std::fill(v.begin(), v.begin() + in.c, absent);
+    if (names_operand(op, i)) {
+      const auto &w = weight(op.in[i]).data;
+      TPUCB_CHECK(w.size() == (size_t)in.c, "group_norm %s: operand %s has %zu values, expected %d", nm, op.in[i].c_str(), w.size(), in.c);
+      std::copy(w.begin(), w.end(), v.begin());
+    }
+    return v;
+  };
+  s.gamma = affine(1, 1.0f);
+  s.beta = affine(2, 0.0f);
+  return s;
+}
+
+// fully_connected whose line names an activation or, as operand 7 behind the quantisation operands, a residual tensor.
+inline bool linear_asked_for(const ParsedOp &op) { return op.attrs.count("activation") || names_operand(op, 7); }
+struct LinearSpec {
+  int m = 0, n = 0, act = ACT_NONE;
+  int hw = 1;         // pixels of an input row: K is hw x channels
+  int k_dev = 0;      // K on the device, with the input's channel pitch
+  std::vector<float> bias; // with the result's channel pitch
+  const HostWeight *filter = nullptr;
+};
+inline LinearSpec linear_spec(const ParsedOp &op, const DevTensor &in, const DevTensor &out, const DevTensor *res, const WeightOf &weight) {
+  const char *nm = op.name.c_str();
+  TPUCB_CHECK(in.dtype == out.dtype && out.dtype != 0, "fc %s: activation and residual need a BF16 or fp32 input and a result of its type", nm);
+  LinearSpec s;
+  s.act = activation_from_string(op.gets("activation", "none"), "fc " + op.name);
+  if (op.geti("do_relu", 0)) {
+    TPUCB_CHECK(!op.attrs.count("activation"), "fc %s: do_relu and activation exclude each other", nm);
+    s.act = ACT_RELU;
+  }
+  TPUCB_CHECK(names_operand(op, 1), "fc %s: expects input, filter[, bias, -, -, -, -, residual]", nm);
+  s.filter = &weight(op.in[1]);
+  TPUCB_CHECK(s.filter->shape.size() <= 2, "fc %s: batched inner products have no activation or residual", nm);
+  s.m = in.n;
+  s.n = out.c;
+  TPUCB_CHECK(in.n > 0 && in.c > 0 && in.h > 0 && in.w > 0 && out.c > 0, "fc %s: empty input or result", nm);
+  TPUCB_CHECK((double)in.h * in.w * in.cp < (double)(1 << 29), "fc %s: input rows are too long", nm);
+  TPUCB_CHECK(!in.padded_rows() && out.n == in.n && out.h == 1 && out.w == 1, "fc %s: output must be [m, n]", nm);
+  s.hw = in.h * in.w;
+  s.k_dev = s.hw * in.cp;
+  const size_t k = (size_t)in.c * s.hw;
+  TPUCB_CHECK(s.filter->data.size() == s.n * k, "fc %s: filter has %zu values, expected n*k = %zu", nm, s.filter->data.size(), s.n * k);
+  s.bias.assign(out.cp, 0.0f);
+  if (names_operand(op, 2)) {
+    const auto &b = weight(op.in[2]).data;
+    TPUCB_CHECK(b.size() == (size_t)s.n, "fc %s: bias has %zu values, expected %d", nm, b.size(), s.n);
+    std::copy(b.begin(), b.end(), s.bias.begin());
+  }
+  if (res)
+    TPUCB_CHECK(res->dtype == out.dtype && res->n == out.n && res->c == out.c && res->h == 1 && res->w == 1 && res->cp == out.cp,
+                "fc %s: residual %s must be [%d, %d] of the result's type", nm, op.in[7].c_str(), out.n, out.c);
+  return s;
+}
+
+} // namespace tpucb
