@@ -231,6 +231,48 @@ def test_linear(M, k, dtype):
     assert_close(run_linear(M, x, w, bias, act, res, dtype), want, tol, "%s %s %s" % (LINEAR_CASES[k], act, dtype))
 
 
+@pytest.mark.parametrize("tiles", [1016, 1032, 1064, 1128, 1256, 2016, 2064, 3048, 4112, 4256, 5080, 7128, 8016, 8128, 8256, 10032, 10064, 10128, 10192, 10256])
+@pytest.mark.parametrize("m,k,n", [(1, 600, 300), (33, 1000, 130), (200, 520, 272), (300, 4160, 530), (515, 64, 1040)])
+def test_linear_tensor_core_forms(M, m, k, n, tiles):
+    """Every form of the tensor-core kernels on every size, whatever the rule by size would take."""
+    rng = np.random.default_rng(m + n)
+    x, w = cast(rng.normal(0, 1, (m, k)), "BF16"), cast(rng.normal(0, k ** -0.5, (n, k)), "BF16")
+    bias, res = rng.normal(0, 0.3, n).astype(np.float32), cast(rng.normal(0, 1, (m, n)), "BF16")
+    want, tol = linear_want(x, w, bias, "silu", res, "BF16")
+    form = {}
+    got = run_linear(M, x, w, bias, "silu", res, options=[("linear_tiles", tiles)], form=form)
+    pair = tiles >= 10000
+    assert form == {"tiles": "pair" if pair else "cluster", "channels": tiles % 1000, "split_k": 1 if pair else min(tiles // 1000, (k + 63) // 64)}
+    assert_close(got, want, tol)
+    assert np.array_equal(got, run_linear(M, x, w, bias, "silu", res, options=[("linear_tiles", tiles)]))
+
+
+@pytest.mark.parametrize("tiles", [1128, 4064, 10064])
+def test_linear_bounded_wait_runs_out(M, tiles):
+    """A hand-over that never comes: the launch ends with a status, the interpreter stays usable."""
+    from tpu_compiler_b200 import TpucbError
+    rng = np.random.default_rng(19)
+    m, k, n = 700, 512, 2048  # 96 tiles of a pair: some do the third, which needs an accumulator back
+    n = 8192 if tiles >= 10000 else n
+    x, w = cast(rng.normal(0, 1, (m, k)), "BF16"), cast(rng.normal(0, k ** -0.5, (n, k)), "BF16")
+    text = "input name=x shape=%d,%d dtype=BF16\nfully_connected name=y in=x,f shape=%d,%d dtype=BF16 activation=relu\n" % (m, k, m, n)
+    mod = M(0)
+    mod.set_option("linear_tiles", tiles)
+    for rounds in (4, 0):
+        mod.set_option("selftest_lost_arrival", rounds)
+        mod.load_text(text, {"f": w})
+        mod.set_tensor("x", x)
+        if rounds:
+            for _ in range(2):
+                with pytest.raises(TpucbError, match="bounded wait"):
+                    mod.invoke()
+        else:
+            mod.invoke()
+    want, tol = linear_want(x, w, None, "relu", None, "BF16")
+    assert_close(mod.get_tensor("y"), want, tol)
+    mod.close()
+
+
 @pytest.mark.parametrize("dtype", ["BF16", "FP32"])
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("m,n", [(3, 40), (200, 144)])

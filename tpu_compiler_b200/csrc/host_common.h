@@ -116,30 +116,41 @@ struct PdlConvScope {
 // attribute: the kernel may be scheduled while its predecessor in the stream is still running and orders itself
 // behind it with pdl_wait (every kernel launched this way begins with pdl_prologue or places pdl_wait itself).
 template <typename... KArgs, typename G, typename B, typename... Args>
-inline void launch_k(void (*kernel)(KArgs...), G grid, B block, size_t smem, cudaStream_t stream, Args &&...args) {
+inline void launch_cluster_k(unsigned cluster, void (*kernel)(KArgs...), G grid, B block, size_t smem, cudaStream_t stream, Args &&...args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(block);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
   // Mode 1 marks small launches of the other kernels too: one that has no more than a block's worth of threads per SM
   // cannot be placed badly by the order in which its predecessor's blocks leave, and its scheduling is most of what it
   // costs (MobileNet-v2 batch 1 227 -> 218 us, 12 307 -> 296; YOLOv4-style batch 1 1181 -> 1160; twice the threads: a loss).
   const bool pdl = launch_pdl_flag() || (pdl_mode() == 1 && (size_t)cfg.gridDim.x * cfg.gridDim.y * cfg.gridDim.z *
                                              cfg.blockDim.x * cfg.blockDim.y * cfg.blockDim.z <= (size_t)launch_sm_count() * 256);
-  // The arguments are converted to the kernel's own parameter types and passed by address; without the attribute the
+  cudaLaunchAttribute attr[2];
+  cfg.attrs = attr;
+  if (pdl) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) { // blocks of a cluster, along x (kernels that fix theirs pass 1)
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = cluster;
+    attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  // The arguments are converted to the kernel's own parameter types and passed by address; without an attribute the
   // launch goes through the classic entry point.
   auto go = [&](KArgs... a) {
     void *pa[sizeof...(KArgs) + 1] = {(void *)&a...};
-    return pdl ? cudaLaunchKernelExC(&cfg, (const void *)kernel, pa)
-               : cudaLaunchKernel((const void *)kernel, cfg.gridDim, cfg.blockDim, pa, smem, stream);
+    return cfg.numAttrs ? cudaLaunchKernelExC(&cfg, (const void *)kernel, pa)
+                        : cudaLaunchKernel((const void *)kernel, cfg.gridDim, cfg.blockDim, pa, smem, stream);
   };
   TPUCB_CUDA(go(std::forward<Args>(args)...));
+}
+template <typename Kernel, typename G, typename B, typename... Args>
+inline void launch_k(Kernel kernel, G grid, B block, size_t smem, cudaStream_t stream, Args &&...args) {
+  launch_cluster_k(1, kernel, grid, block, smem, stream, std::forward<Args>(args)...);
 }
 #endif
 

@@ -14,6 +14,7 @@
 #include "extra_kernels.cuh"
 #include "group_norm.cuh"
 #include "linear.cuh"
+#include "linear_tc.cuh"
 #include "module_text.h"
 
 #include <algorithm>
@@ -249,6 +250,7 @@ public:
   bool fuse_activations = true; // set before load_module
   int big_tiles = 1; // set before load_module: see conv_big_mode
   int fuse_residual_add = 2; // set before load_module: eltwise adds in the producing convolution's epilogue: 0 never, 1 always, 2 by size
+  int linear_tiles = 1; // set before load_module: see linear_tc_plan
   bool fp32_tensor_cores = true; // set before load_module: fp32 convolutions as three TF32 products
   void link_tf32_remainders();
   void fuse_activation_chains(const std::map<std::string, int> &uses);
@@ -1908,15 +1910,40 @@ public:
       return (const void *)I.upload(w);
     };
     a_.w = out->dtype == DT_F32 ? packed(0.0f, [](float v) { return v; }) : packed((uint16_t)0, [](float v) { return f32_to_bf16_bits(v); });
+    if (out->dtype == DT_BF16) {
+      tc_.plan = linear_tc_plan(s.m, s.k_dev, out->cp, I.sm_count, I.linear_tiles);
+      const LinearTcPlan &l = tc_.plan;
+      LinearTcParams &p = tc_.p;
+      p = LinearTcParams{};
+      p.m = s.m; p.n_pad = p.ldy = out->cp;
+      p.k_blocks = l.k_blocks; p.nt = l.nt; p.split = l.split; p.a_rows = l.a_rows; p.stages = l.stages; p.tmem_cols = l.tmem_cols;
+      p.idesc = make_idesc_bf16(l.pair ? 256 : 128, l.nt);
+      p.bias = a_.bias;
+      p.res = (const uint16_t *)a_.res;
+      p.y = (uint16_t *)a_.y;
+      p.err = &I.ss.d_err->code;
+      p.wait_rounds = I.selftest_lost_arrival;
+      p.lose_arrival = I.selftest_lost_arrival > 0;
+      encode_matrix_map(&tc_.tmX, (const int8_t *)in->dev, s.m, s.k_dev * 2, s.k_dev * 2, 128, l.pair ? 128 : l.a_rows);
+      encode_matrix_map(&tc_.tmW, (const int8_t *)a_.w, out->cp, s.k_dev * 2, s.k_dev * 2, 128, l.pair ? l.nt / 2 : l.nt);
+      linear_kernel_ready(tc_, act_);
+    }
     alg_ops = 2.0 * s.m * k * s.n;
     alg_bytes = (double)out->elsize() * ((double)s.m * k + (double)s.n * k + (double)s.m * s.n * (res_ ? 2 : 1)) + 4.0 * s.n;
   }
-  void invoke(cudaStream_t s) override { launch_linear(a_, out_->dtype == DT_F32, act_, s); }
-  std::string form() const override { return "tiles=direct"; }
+  void invoke(cudaStream_t s) override {
+    if (out_->dtype == DT_BF16) launch_linear_tc(tc_, act_, s);
+    else launch_linear(a_, true, act_, s);
+  }
+  std::string form() const override {
+    if (out_->dtype != DT_BF16) return "tiles=direct";
+    return std::string("tiles=") + (tc_.plan.pair ? "pair" : "cluster") + " channels=" + std::to_string(tc_.plan.nt) + " split_k=" + std::to_string(tc_.plan.split);
+  }
 
 private:
   TensorPtr in_, out_, res_;
   LinearArgs a_;
+  LinearTc tc_;
   int act_ = ACT_NONE;
 };
 

@@ -97,4 +97,52 @@ inline LinearSpec linear_spec(const ParsedOp &op, const DevTensor &in, const Dev
   return s;
 }
 
+// ---- how an inner product runs on the tensor cores (linear_tc.cuh)
+constexpr int kLinearMaxStages = 16;
+constexpr int kLinearHeader = 1024; // barriers
+struct LinearTcPlan {
+  bool pair = false;  // two SMs per tile of 256 rows, persistent; else one of 128, and `split` CTAs share its K
+  int nt = 0, split = 1, a_rows = 128, stages = 0, k_blocks = 0;
+  unsigned tmem_cols = 512, grid = 0;
+  size_t smem = 0;
+};
+// The sizes that follow from tiles of `nt` channels whose K is shared by `split` CTAs, or tiles of a pair.
+inline LinearTcPlan linear_tc_sizes(bool pair, int nt, int split, int m, int k_dev, int n_pad, int sm_count) {
+  LinearTcPlan l;
+  l.pair = pair;
+  l.nt = nt;
+  l.k_blocks = (k_dev + 63) / 64;
+  l.split = pair ? 1 : std::min(split, l.k_blocks);
+  const long long n_tiles = (n_pad + nt - 1) / nt;
+  if (pair) {
+    const size_t stage = (size_t)(128 + nt / 2) * 128;
+    const long long tiles = n_tiles * ((m + 255) / 256);
+    l.stages = (int)std::min<size_t>(kLinearMaxStages, (226 * 1024 - kLinearHeader - 1024) / stage);
+    l.smem = 1024 + kLinearHeader + l.stages * stage; // (more than half of an SM's: two pairs on the same SMs would wait for each other's tensor memory)
+    l.grid = (unsigned)(2 * std::min<long long>(tiles, sm_count / 2));
+    return l;
+  }
+  l.a_rows = std::min(128, round_up(m, 8));
+  l.tmem_cols = 32;
+  while ((int)l.tmem_cols < nt) l.tmem_cols *= 2;
+  const size_t stage = (size_t)round_up(l.a_rows * 128, 1024) + (size_t)round_up(nt * 128, 1024);
+  const int blocks = (l.k_blocks + l.split - 1) / l.split;
+  // half of an SM's shared memory: two CTAs share it, one's epilogue beside the other's loop
+  l.stages = std::max(1, (int)std::min<size_t>(std::min(blocks, kLinearMaxStages), (112 * 1024 - kLinearHeader - 1024) / stage));
+  size_t ring = l.stages * stage;
+  ring = std::max(ring, (l.stages - 1) * stage + 128 * 128);                                    // the tensor core reads 128 rows of the last stage
+  if (l.split > 1) ring = std::max(ring, (size_t)nt * std::min(128, round_up(m, 32)) * 4); // the exchange of partial sums
+  l.smem = 1024 + kLinearHeader + ring;
+  l.grid = (unsigned)(n_tiles * ((m + 127) / 128) * l.split);
+  return l;
+}
+// mode (option "linear_tiles"): 1 by size; 1000 * split + nt; 10000 + nt: pairs
+inline LinearTcPlan linear_tc_plan(int m, int k_dev, int n_pad, int sm_count, int mode) {
+  if (mode >= 10000) return linear_tc_sizes(true, mode - 10000, 1, m, k_dev, n_pad, sm_count);
+  if (mode >= 1000) return linear_tc_sizes(false, mode % 1000, mode / 1000, m, k_dev, n_pad, sm_count);
+  const long long tiles = (long long)((m + 255) / 256) * ((n_pad + 255) / 256);
+  if (tiles >= sm_count / 3) return linear_tc_sizes(true, 256, 1, m, k_dev, n_pad, sm_count);
+  return linear_tc_sizes(false, 64, 2, m, k_dev, n_pad, sm_count);
+}
+
 } // namespace tpucb
