@@ -66,7 +66,7 @@ def norm_want(x, groups, gamma, beta, eps, act, dtype):
     return y.reshape(x.shape), tol.reshape(x.shape)
 
 
-def run_norm(M, x, groups, gamma, beta, eps=1e-5, act="none", dtype="BF16", options=()):
+def run_norm(M, x, groups, gamma, beta, eps=1e-5, act="none", dtype="BF16", options=(), form=None):
     w, ins = {}, ["x"]
     for name, v in (("ga", gamma), ("be", beta)):
         ins.append("-" if v is None else name)
@@ -77,6 +77,8 @@ def run_norm(M, x, groups, gamma, beta, eps=1e-5, act="none", dtype="BF16", opti
         m.set_option(k, v)
     m.load_text("input name=x shape=%s dtype=%s\ngroup_norm name=y in=%s shape=%s dtype=%s groups=%d variance_epsilon=%g activation=%s\n" % (
         dims(x.shape), dtype, ",".join(ins), dims(x.shape), dtype, groups, eps, act), w)
+    if form is not None:
+        form.update(m.op_form("y"))
     m.set_tensor("x", x)
     m.invoke()
     got = m.get_tensor("y")
@@ -107,6 +109,35 @@ def test_group_norm(M, k, dtype):
     act = ACTS[k % 5]
     want, tol = norm_want(x, groups, gamma, beta, 1e-5, act, dtype)
     assert_close(run_norm(M, x, groups, gamma, beta, act=act, dtype=dtype), want, tol, "%s %d %s %s" % (shape, groups, act, dtype))
+
+
+NORM_FORMS = ["rows_warp", "rows_block", "slab", "streamed", "strided"]
+
+
+@pytest.mark.parametrize("dtype", ["BF16", "FP32"])
+@pytest.mark.parametrize("form,shape,groups", [(f, s, g) for s, g, forms in [
+    ((37, 200), 1, "rows_warp rows_block slab streamed strided"), ((37, 203), 1, "rows_warp rows_block slab streamed strided"),
+    ((5, 640), 16, "rows_warp rows_block slab streamed strided"), ((130, 1000), 1, "rows_warp rows_block slab streamed strided"),
+    ((3, 6001), 1, "rows_block strided"), ((2, 33, 5, 7), 11, "slab streamed strided"), ((2, 64, 40, 41), 8, "slab streamed strided"),
+    ((2, 40, 40, 41), 4, "slab streamed strided"), ((1, 17, 30, 100), 1, "slab streamed strided"), ((3, 96, 3, 1), 96, "slab streamed strided"),
+    ((1, 512, 60, 77), 32, "slab streamed strided"), ((4, 2048, 2, 2), 32, "slab streamed strided"), ((1, 64, 200, 203), 2, "streamed strided"),
+    ((1, 4100, 3, 3), 4, "strided")] for f in forms.split()])
+def test_group_norm_forms(M, form, shape, groups, dtype):
+    """Every form on every tensor that it can take, whatever the rule by size would choose."""
+    rng = np.random.default_rng(30)
+    per = [1, shape[1]] + [1] * (len(shape) - 2)
+    x = cast(rng.normal(0, 1, shape) * np.exp(rng.normal(0, 0.5, per)) + rng.normal(0, 1, per), dtype)
+    gamma, beta = rng.normal(1, 0.3, shape[1]).astype(np.float32), rng.normal(0, 0.3, shape[1]).astype(np.float32)
+    want, tol = norm_want(x, groups, gamma, beta, 1e-5, "silu", dtype)
+    took = {}
+    options = [("norm_form", 1 + NORM_FORMS.index(form))]
+    got = run_norm(M, x, groups, gamma, beta, act="silu", dtype=dtype, options=options, form=took)
+    assert took["form"] == form
+    assert_close(got, want, tol)
+    assert np.array_equal(got, run_norm(M, x, groups, gamma, beta, act="silu", dtype=dtype, options=options))
+    hard = cast(rng.normal(0, 1, shape) + 500.0, dtype)  # a mean far from zero
+    want, tol = norm_want(hard, groups, None, None, 1e-5, "none", dtype)
+    assert_close(run_norm(M, hard, groups, None, None, dtype=dtype, options=options), want, tol)
 
 
 @pytest.mark.parametrize("dtype", ["BF16", "FP32"])

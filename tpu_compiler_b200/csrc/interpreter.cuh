@@ -250,6 +250,7 @@ public:
   bool fuse_activations = true; // set before load_module
   int big_tiles = 1; // set before load_module: see conv_big_mode
   int fuse_residual_add = 2; // set before load_module: eltwise adds in the producing convolution's epilogue: 0 never, 1 always, 2 by size
+  int norm_form = 0;    // set before load_module: see group_norm_plan
   int linear_tiles = 1; // set before load_module: see linear_tc_plan
   bool fp32_tensor_cores = true; // set before load_module: fp32 convolutions as three TF32 products
   void link_tf32_remainders();
@@ -1954,17 +1955,34 @@ class GroupNormOp : public OpKernel {
 public:
   GroupNormOp(Interpreter &I, const ParsedOp &op, TensorPtr in, TensorPtr out) : in_(in), out_(out) {
     const GroupNormSpec s = group_norm_spec(op, *in, *out, [&](const std::string &nm) -> const HostWeight & { return I.weight(nm); });
-    act_ = s.act;
-    a_ = GroupNormArgs{in->dev, out->dev, I.upload(s.gamma), I.upload(s.beta), in->n, in->h * in->w, in->c, in->cp, s.groups, in->c / s.groups, s.eps};
+    plan_ = group_norm_plan(in->n, in->h * in->w, in->c, s.groups, (int)in->elsize(), I.sm_count, I.norm_form);
+    a_ = GroupNormArgs{};
+    a_.in = in->dev; a_.out = out->dev;
+    a_.gamma = I.upload(s.gamma); a_.beta = I.upload(s.beta);
+    a_.n = in->n; a_.pixels = in->h * in->w; a_.c = in->c; a_.cp = in->cp; a_.groups = s.groups; a_.cg = in->c / s.groups;
+    a_.eps = s.eps; a_.act = s.act;
+    a_.vecs = plan_.vecs; a_.chunk_groups = plan_.chunk_groups; a_.chunks = plan_.chunks; a_.parts = plan_.parts; a_.part_pixels = plan_.part_pixels;
+    if (plan_.form == NORM_STREAMED) {
+      const size_t rows = (size_t)in->n * s.groups, counters = (size_t)in->n * plan_.chunks;
+      a_.partial = (float2 *)I.dalloc(rows * plan_.parts * sizeof(float2));
+      a_.stats = (float2 *)I.dalloc(rows * sizeof(float2));
+      a_.arrived = (unsigned *)I.dalloc(counters * sizeof(unsigned));
+      TPUCB_CUDA(cudaMemsetAsync(a_.arrived, 0, counters * sizeof(unsigned), I.stream));
+    }
     alg_ops = 8.0 * in->numel();
     alg_bytes = 2.0 * in->numel() * in->elsize() + 8.0 * in->c;
   }
-  void invoke(cudaStream_t s) override { launch_group_norm(a_, out_->dtype == DT_F32, act_, s); }
+  void invoke(cudaStream_t s) override { launch_group_norm(a_, plan_, out_->dtype == DT_F32, s); }
+  int kernel_launches() const override { return plan_.form == NORM_STREAMED ? 2 : 1; }
+  std::string form() const override {
+    static const char *names[] = {"rows_warp", "rows_block", "slab", "streamed", "strided"};
+    return std::string("form=") + names[plan_.form] + " parts=" + std::to_string(plan_.parts);
+  }
 
 private:
   TensorPtr in_, out_;
   GroupNormArgs a_;
-  int act_ = ACT_NONE;
+  GroupNormPlan plan_;
 };
 
 // ====================================================================== Interpreter bodies

@@ -392,6 +392,9 @@ int tpucb_interp_set_option(tpucb_interp *it, const char *key, int value) {
     TPUCB_CHECK(value == 0 || value == 1 || ((value / 1000 == 1 || value / 1000 == 2) && px >= 32 && px <= 256 && px % 32 == 0),
                 "big_tiles: 0 (never), 1 (by size, the default) or 1000 * CTAs (1, 2) + pixels (32 .. 256, a multiple of 32)");
     it->impl.big_tiles = value; // takes effect at the next load_module
+  } else if (k == "norm_form") {
+    TPUCB_CHECK(value >= 0 && value <= 5, "norm_form: 0 (by size, the default) or 1 to 5: rows by warps, rows by blocks, slab, streamed, strided, where a tensor can");
+    it->impl.norm_form = value; // takes effect at the next load_module
   } else if (k == "linear_tiles") {
     const int nt = value >= 10000 ? value - 10000 : value % 1000, split = value / 1000;
     TPUCB_CHECK(value == 1 || (value >= 10000 ? nt >= 32 && nt <= 256 && nt % 32 == 0 : split >= 1 && split <= 8 && nt >= 16 && nt <= 256 && nt % 16 == 0),
