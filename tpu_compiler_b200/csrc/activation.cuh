@@ -24,41 +24,80 @@ __device__ __forceinline__ float rcp_approx(float v) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
-// v / (1 + e^-s): an overflowing exponential gives a quotient of zero, as it should
-__device__ __forceinline__ float times_sigmoid(float v, float s) { return v * rcp_approx(1.0f + ex2_approx(s * -1.4426950408889634f)); }
+
+// Two values in a register pair: the packed instructions round each half as the single ones do and take one issue slot for two.
+struct Pair {
+  unsigned long long v;
+  __device__ __forceinline__ Pair() {}
+  __device__ __forceinline__ Pair(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi)); }
+  __device__ __forceinline__ float lo() const { return __uint_as_float((uint32_t)v); }
+  __device__ __forceinline__ float hi() const { return __uint_as_float((uint32_t)(v >> 32)); }
+};
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+  Pair d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+  Pair d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
+  Pair d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return d;
+}
+__device__ __forceinline__ Pair both(float v) { return Pair(v, v); }
+// two BF16 values of a word
+__device__ __forceinline__ Pair pair_of_bf16(uint32_t w) { return Pair(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+
+// 1 / a of each half with one reciprocal: 1 / lo = hi / (lo hi). The special-function unit (16 results per clock and SM) bounds
+// the activations of memory-bound passes: 2 results per value are 30 us for 2^26 values on 148 SMs, 1.5 are 22. |lo hi| must stay in
+// range.
+__device__ __forceinline__ Pair reciprocals(Pair a) {
+  const float r = rcp_approx(a.lo() * a.hi());
+  return Pair(a.hi(), a.lo()) * both(r);
+}
+// v / (1 + 2^t). The exponent is held at 60, so that the product of two denominators stays in range: what is cut off is below
+// 2^-60 of v.
+__device__ __forceinline__ Pair over_one_plus_exp2(Pair v, Pair t) {
+  return v * reciprocals(Pair(ex2_approx(fminf(t.lo(), 60.0f)), ex2_approx(fminf(t.hi(), 60.0f))) + both(1.0f));
+}
 
 // gelu(v) = v Phi(v) = max(v, 0) - |v| Q(|v|), with the upper tail of the normal distribution Q(a) = erfc(a / sqrt 2) / 2 =
 // e^(-a^2/2) P(1 / (1 + p a)): no cancellation on either side. The polynomials P are this file's own minimax fits of
 // e^(a^2/2) Q(a) over a in [0, 14] (beyond, Q is below 1e-44): largest relative error 2.4e-5 for BF16 results, a hundredth of
-// their rounding, and 3.1e-7 for fp32 ones.
-template <bool F32> __device__ __forceinline__ float gelu_exact(float v) {
-  const float a = fabsf(v), t = rcp_approx(fmaf(0.35f, a, 1.0f)), e = ex2_approx(a * a * -0.7213475204444817f);
-  float q;
+// their rounding, and 3.1e-7 for fp32 ones. (Beyond 2^40 the reciprocals of a pair would leave the range: a is held there.)
+template <bool F32> __device__ __forceinline__ Pair gelu_exact(Pair v) {
+  const Pair a(fminf(fabsf(v.lo()), 1.0995116e12f), fminf(fabsf(v.hi()), 1.0995116e12f));
+  const Pair t = reciprocals(fma(both(0.35f), a, both(1.0f))), x = a * a * both(-0.7213475204444817f);
+  const Pair e(ex2_approx(x.lo()), ex2_approx(x.hi()));
+  Pair q;
   if (F32) {
-    q = 0.04894244623667017f;
-    q = fmaf(q, t, -0.2021192868271973f);
-    q = fmaf(q, t, 0.24064081895892164f);
-    q = fmaf(q, t, -0.01702343620260618f);
-    q = fmaf(q, t, 0.15596148733152987f);
-    q = fmaf(q, t, 0.13335509625098455f);
-    q = fmaf(q, t, 0.14027034361266144f);
-    q = fmaf(q, t, -2.731554772757582e-05f);
+    q = fma(both(0.04894244623667017f), t, both(-0.2021192868271973f));
+    q = fma(q, t, both(0.24064081895892164f));
+    q = fma(q, t, both(-0.01702343620260618f));
+    q = fma(q, t, both(0.15596148733152987f));
+    q = fma(q, t, both(0.13335509625098455f));
+    q = fma(q, t, both(0.14027034361266144f));
+    q = fma(q, t, both(-2.731554772757582e-05f));
   } else {
-    q = -0.09778110211354195f;
-    q = fmaf(q, t, 0.278881467362648f);
-    q = fmaf(q, t, 0.010946683641198824f);
-    q = fmaf(q, t, 0.17298857188677733f);
-    q = fmaf(q, t, 0.13469103084119843f);
-    q = fmaf(q, t, 0.0002850549969567228f);
+    q = fma(both(-0.09778110211354195f), t, both(0.278881467362648f));
+    q = fma(q, t, both(0.010946683641198824f));
+    q = fma(q, t, both(0.17298857188677733f));
+    q = fma(q, t, both(0.13469103084119843f));
+    q = fma(q, t, both(0.0002850549969567228f));
   }
-  return fmaxf(v, 0.0f) - a * (q * e);
+  // (fmaxf would lose a NaN)
+  return fma(a * both(-1.0f), q * e, Pair(v.lo() < 0.0f ? 0.0f : v.lo(), v.hi() < 0.0f ? 0.0f : v.hi()));
 }
-template <int ACT, bool F32> __device__ __forceinline__ float activate(float v) {
-  if (ACT == ACT_RELU) return v < 0.0f ? 0.0f : v;
-  if (ACT == ACT_SILU) return times_sigmoid(v, v);
+template <int ACT, bool F32> __device__ __forceinline__ Pair activate(Pair v) {
+  if (ACT == ACT_RELU) return Pair(v.lo() < 0.0f ? 0.0f : v.lo(), v.hi() < 0.0f ? 0.0f : v.hi());
+  if (ACT == ACT_SILU) return over_one_plus_exp2(v, v * both(-1.4426950408889634f));
   if (ACT == ACT_GELU) return gelu_exact<F32>(v);
   // 0.5 v (1 + tanh u) = v / (1 + e^(-2u)), u = sqrt(2 / pi) (v + 0.044715 v^3)
-  if (ACT == ACT_GELU_TANH) return times_sigmoid(v, v * fmaf(0.07135481627159882f, v * v, 1.5957691216057308f));
+  if (ACT == ACT_GELU_TANH) return over_one_plus_exp2(v, v * fma(v * v, both(-0.10294324f), both(-2.3022082f)));
   return v;
 }
 // `use` is called with the activation as a compile-time constant

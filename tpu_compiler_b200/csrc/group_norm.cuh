@@ -8,13 +8,15 @@
 //   rows     one pixel per image: a group is contiguous; a warp or a block keeps it in registers;
 //   slab     the pixels of an image x a few groups ("chunk") are kept in the registers of a cluster of up to eight blocks, which
 //            exchange their statistics through shared memory: x is read once;
-//   streamed larger ones: a pass for the statistics, whose last block per chunk joins the partial ones, and a pass that forms
-//            the results, in the opposite order, so that it begins with what the L2 still holds;
+//   streamed larger ones: a pass for the statistics of parts of an image, and a pass that joins them and forms the results, in the
+//            opposite order, so that it begins with what the L2 still holds;
 //   strided  what fits no whole vectors: a block per group, three passes.
-// Variances are never differences of large sums: rows and slab take the mean first and then the squares of the distances from it, out of
-// the registers; streamed sums distances from the first value that a thread sees of a channel (the error is then at most the
-// thread's count times 2^-24 of the variance, even where that value is an outlier: it is part of the variance). Partial ones are joined as
+// Variances are never differences of large sums. Rows and slab take the mean first and then the squares of the distances from it, out
+// of the registers (slab: from the mean of the block). Streamed sums distances from the first value that a thread sees in a channel, and
+// their squares: the error is then at most the thread's count times 2^-24 of the variance, even where that value is an outlier (it is part
+// of the variance; one such value for the whole block cost 1e-4 of it). Partial ones are joined as
 //   M2 = sum M2_i + sum n_i (mean_i - mean)^2.
+// The result is one multiply-add per value, with beta - mean rstd gamma rounded once, an error like that of the mean itself.
 #pragma once
 #include "activation.cuh"
 #include "conv_big.cuh"
@@ -29,78 +31,70 @@ struct GroupNormArgs {
   float eps;
   int act;
   // slab and streamed: chunks of `vecs` vectors = whole groups (the last may have fewer), `parts` blocks share an image's pixels
-  int vecs, chunk_groups, chunks, parts, part_pixels;
-  float2 *partial;    // streamed: [n][groups][parts] mean, M2
-  float2 *stats;      // streamed: [n][groups] mean, 1 / sqrt(var + eps)
-  unsigned *arrived;  // streamed: [n][chunks], zero between launches
+  int vecs, lanes, chunk_groups, chunks, parts, part_pixels; // (lanes: pixels that a block's threads take at once)
+  int apply_parts, apply_pixels; // streamed: of the second pass
+  int col_split;                 // norm_group_sums: threads per column, max(1, threads / columns)
+  float inv_vecs, inv_lanes, inv_cg, inv_width;        // 1 / vecs and so on, for quotients of small numbers (small_div)
+  float2 *partial;               // streamed: [n][groups][parts] mean, M2
 };
+// a / b for a < 2^22, given 1 / b: a + 1/2 is at least 1 / (2 b) of a quotient away from the next whole one, and the product's error less
+__device__ __forceinline__ int small_div(int a, float inv_b) { return (int)(((float)a + 0.5f) * inv_b); }
 
-// Sixteen bytes of values
+// Sixteen bytes of values, as pairs
 template <typename T> struct NormVec;
 template <> struct NormVec<float> {
-  static constexpr int N = 4;
+  static constexpr int N = 4, P = 2;
   static constexpr bool kF32 = true;
-  static __device__ __forceinline__ void get(const uint4 &r, float (&v)[4]) {
-    v[0] = __uint_as_float(r.x);
-    v[1] = __uint_as_float(r.y);
-    v[2] = __uint_as_float(r.z);
-    v[3] = __uint_as_float(r.w);
+  static __device__ __forceinline__ void get(const uint4 &r, Pair (&v)[2]) {
+    v[0] = Pair(__uint_as_float(r.x), __uint_as_float(r.y));
+    v[1] = Pair(__uint_as_float(r.z), __uint_as_float(r.w));
   }
-  static __device__ __forceinline__ uint4 put(const float (&v)[4]) {
-    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  static __device__ __forceinline__ uint4 put(const Pair (&v)[2]) {
+    return make_uint4(__float_as_uint(v[0].lo()), __float_as_uint(v[0].hi()), __float_as_uint(v[1].lo()), __float_as_uint(v[1].hi()));
   }
   static __device__ __forceinline__ float one(float v) { return v; }
   static __device__ __forceinline__ float back(float v) { return v; }
 };
 template <> struct NormVec<uint16_t> {
-  static constexpr int N = 8;
+  static constexpr int N = 8, P = 4;
   static constexpr bool kF32 = false;
-  static __device__ __forceinline__ void get(const uint4 &r, float (&v)[8]) {
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = __uint_as_float(w[i] << 16);
-      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
+  static __device__ __forceinline__ void get(const uint4 &r, Pair (&v)[4]) {
+    v[0] = pair_of_bf16(r.x);
+    v[1] = pair_of_bf16(r.y);
+    v[2] = pair_of_bf16(r.z);
+    v[3] = pair_of_bf16(r.w);
   }
-  static __device__ __forceinline__ uint4 put(const float (&v)[8]) {
-    return make_uint4(bf16x2_ieee(v[0], v[1]), bf16x2_ieee(v[2], v[3]), bf16x2_ieee(v[4], v[5]), bf16x2_ieee(v[6], v[7]));
+  static __device__ __forceinline__ uint4 put(const Pair (&v)[4]) {
+    return make_uint4(bf16x2_ieee(v[0].lo(), v[0].hi()), bf16x2_ieee(v[1].lo(), v[1].hi()), bf16x2_ieee(v[2].lo(), v[2].hi()),
+                      bf16x2_ieee(v[3].lo(), v[3].hi()));
   }
   static __device__ __forceinline__ float one(uint16_t v) { return bf16_bits_to_f32(v); }
   static __device__ __forceinline__ uint16_t back(float v) { return (uint16_t)bf16x2_ieee(v, v); }
 };
 
 // the activation of a vector's values; which one is the same for the whole launch
-template <bool F32, int N> __device__ __forceinline__ void activate_all(int act, float (&v)[N]) {
-  switch (act) {
-  case ACT_RELU:
+template <bool F32, int P> __device__ __forceinline__ void activate_all(int act, Pair (&v)[P]) {
+  auto each = [&](auto k) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = activate<ACT_RELU, F32>(v[j]);
-    break;
-  case ACT_SILU:
+    for (int j = 0; j < P; ++j) v[j] = activate<decltype(k)::value, F32>(v[j]);
+  };
+  if (act == ACT_RELU) each(std::integral_constant<int, ACT_RELU>());
+  else if (act == ACT_SILU) each(std::integral_constant<int, ACT_SILU>());
+  else if (act == ACT_GELU) each(std::integral_constant<int, ACT_GELU>());
+  else if (act == ACT_GELU_TANH) each(std::integral_constant<int, ACT_GELU_TANH>());
+}
+template <int P> __device__ __forceinline__ void load_floats(const float *p, Pair (&v)[P]) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = activate<ACT_SILU, F32>(v[j]);
-    break;
-  case ACT_GELU:
-#pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = activate<ACT_GELU, F32>(v[j]);
-    break;
-  case ACT_GELU_TANH:
-#pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = activate<ACT_GELU_TANH, F32>(v[j]);
-    break;
-  default: break;
+  for (int i = 0; i < P / 2; ++i) {
+    const float4 f = __ldg(reinterpret_cast<const float4 *>(p) + i);
+    v[2 * i] = Pair(f.x, f.y);
+    v[2 * i + 1] = Pair(f.z, f.w);
   }
 }
-template <int N> __device__ __forceinline__ void load_floats(const float *p, float (&v)[N]) {
+// zero behind the first `valid` values
+template <int P> __device__ __forceinline__ void clip(Pair (&v)[P], int valid) {
 #pragma unroll
-  for (int i = 0; i < N / 4; ++i) {
-    const float4 f = __ldg(reinterpret_cast<const float4 *>(p) + i);
-    v[4 * i] = f.x;
-    v[4 * i + 1] = f.y;
-    v[4 * i + 2] = f.z;
-    v[4 * i + 3] = f.w;
-  }
+  for (int j = 0; j < P; ++j) v[j] = Pair(2 * j < valid ? v[j].lo() : 0.0f, 2 * j + 1 < valid ? v[j].hi() : 0.0f);
 }
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -117,8 +111,9 @@ __device__ __forceinline__ float block_sum(float v, float *red) {
   return warp_sum(v);
 }
 
-// ---- rows: groups of one pixel. BLOCK: a block per group, else a warp. NV: vectors per thread.
-template <typename T, int NV, bool BLOCK> __global__ void __launch_bounds__(BLOCK ? 1024 : 128) group_norm_rows_kernel(const GroupNormArgs a) {
+// ---- rows: groups of one pixel. BLOCK: a block per group, else a warp. NV: vectors per thread. TAIL: the last vector of a group (there is
+// one group then) ends in padded channels.
+template <typename T, int NV, bool BLOCK, bool TAIL> __global__ void __launch_bounds__(BLOCK ? 512 : 128) group_norm_rows_kernel(const GroupNormArgs a) {
   typedef NormVec<T> V;
   __shared__ float red[32];
   const int lane = BLOCK ? threadIdx.x : threadIdx.x & 31, lanes = BLOCK ? blockDim.x : 32;
@@ -135,345 +130,366 @@ template <typename T, int NV, bool BLOCK> __global__ void __launch_bounds__(BLOC
     const int i = lane + k * lanes;
     raw[k] = i < nvec ? in[i] : make_uint4(0u, 0u, 0u, 0u);
   }
-  // (with one group the last vector may end in padded channels)
-  auto count = [&](int i) { return min(V::N, a.cg - i * V::N); };
-  float s = 0.0f;
+  Pair s2 = both(0.0f);
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    float x[V::N];
+    Pair x[V::P];
     V::get(raw[k], x);
-    const int valid = count(lane + k * lanes);
+    if (TAIL && (lane + k * lanes + 1) * V::N > a.cg) clip(x, a.cg - (lane + k * lanes) * V::N);
 #pragma unroll
-    for (int j = 0; j < V::N; ++j) s += j < valid ? x[j] : 0.0f;
+    for (int j = 0; j < V::P; ++j) s2 = s2 + x[j];
   }
+  float s = s2.lo() + s2.hi();
   s = BLOCK ? block_sum(s, red) : warp_sum(s);
   const float mean = s / (float)a.cg;
-  s = 0.0f;
+  s2 = both(0.0f);
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    float x[V::N];
+    if (lane + k * lanes >= nvec) continue;
+    Pair x[V::P];
     V::get(raw[k], x);
-    const int valid = count(lane + k * lanes);
 #pragma unroll
-    for (int j = 0; j < V::N; ++j) {
-      const float d = j < valid ? x[j] - mean : 0.0f;
-      s = fmaf(d, d, s);
-    }
+    for (int j = 0; j < V::P; ++j) x[j] = x[j] + both(-mean);
+    if (TAIL && (lane + k * lanes + 1) * V::N > a.cg) clip(x, a.cg - (lane + k * lanes) * V::N);
+#pragma unroll
+    for (int j = 0; j < V::P; ++j) s2 = fma(x[j], x[j], s2);
   }
+  s = s2.lo() + s2.hi();
   s = BLOCK ? block_sum(s, red) : warp_sum(s);
   const float rstd = rsqrtf(s / (float)a.cg + a.eps);
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int i = lane + k * lanes;
     if (i >= nvec) continue;
-    float x[V::N], ga[V::N], be[V::N];
+    Pair x[V::P], ga[V::P], be[V::P];
     load_floats(a.gamma + g * a.cg + i * V::N, ga);
     load_floats(a.beta + g * a.cg + i * V::N, be);
     V::get(raw[k], x);
 #pragma unroll
-    for (int j = 0; j < V::N; ++j) x[j] = fmaf((x[j] - mean) * rstd, ga[j], be[j]);
+    for (int j = 0; j < V::P; ++j) x[j] = fma((x[j] + both(-mean)) * both(rstd), ga[j], be[j]);
     activate_all<V::kF32>(a.act, x);
-    const int valid = count(i);
-#pragma unroll
-    for (int j = 0; j < V::N; ++j) x[j] = j < valid ? x[j] : 0.0f;
+    if (TAIL && (i + 1) * V::N > a.cg) clip(x, a.cg - i * V::N);
     out[i] = V::put(x);
   }
 }
 
-// ---- what slab and streamed share: a block of kNormThreads takes pixels x a chunk; a thread keeps to one vector column
-constexpr int kNormThreads = 256;
-template <typename T> struct NormTile {
+// ---- what slab and streamed share: a block takes pixels x a chunk; a thread keeps to one vector column
+template <typename T, int THREADS> struct NormTile { // (parts: of the image, of `pixels` each)
   int img, chunk, part, first_group, n_groups; // groups of this chunk
   int px0, px1;                                // this block's pixels
   int v, p, lanes, ch;                         // the thread's vector column, pixel lane, pixel lanes of the block, first channel
   bool active;
-  __device__ __forceinline__ NormTile(const GroupNormArgs &a, unsigned block) {
-    part = block % a.parts;
-    chunk = (block / a.parts) % a.chunks;
-    img = block / a.parts / a.chunks;
+  __device__ __forceinline__ NormTile(const GroupNormArgs &a, unsigned block, int parts, int pixels) {
+    img = parts == 1 ? block : block / parts;
+    part = block - img * parts;
+    chunk = blockIdx.y;
     first_group = chunk * a.chunk_groups;
     n_groups = min(a.chunk_groups, a.groups - first_group);
-    px0 = part * a.part_pixels;
-    px1 = min(px0 + a.part_pixels, a.pixels);
-    lanes = kNormThreads / a.vecs;
-    p = threadIdx.x / a.vecs;
+    px0 = part * pixels;
+    px1 = min(px0 + pixels, a.pixels);
+    lanes = a.lanes;
+    p = small_div(threadIdx.x, a.inv_vecs);
     v = threadIdx.x - p * a.vecs;
     ch = (chunk * a.vecs + v) * NormVec<T>::N;
     active = p < lanes && ch < a.c;
   }
   __device__ __forceinline__ size_t offset(const GroupNormArgs &a, int px) const { return ((size_t)img * a.pixels + px) * a.cp + ch; }
 };
-// Sums over a chunk's groups of what each thread holds per channel (or, where vectors lie within groups, in all): tab[pixel lane][channel of the
-// chunk], a warp per group. `done(group of the chunk, sum)` in lane 0 of that warp.
-template <int PER, class Done>
-__device__ __forceinline__ void group_sums(const float *tab, int vecs, int lanes, int group_width, int n_groups, Done done) {
-  const int width = vecs * PER;
-  for (int g = threadIdx.x >> 5; g < n_groups; g += kNormThreads / 32) {
+// The block's sum over each group of its chunk of what the threads hold per channel or, where vectors lie within groups (ALIGNED), in
+// all: `done(group of the chunk, sum)` in lane 0 of a warp. tab: THREADS x PER floats, then max(THREADS, columns).
+template <typename T, bool ALIGNED, int THREADS, class Done>
+__device__ __forceinline__ void norm_group_sums(const GroupNormArgs &a, const NormTile<T, THREADS> &t, const Pair *x, float *tab, Done done) {
+  typedef NormVec<T> V;
+  constexpr int PER = ALIGNED ? 1 : V::N;
+  const int width = a.vecs * PER; // columns: vectors or channels
+  const int split = a.col_split; // threads per column
+  float *cols = tab + THREADS * PER;
+  if constexpr (ALIGNED) {
+    tab[threadIdx.x] = x[0].lo() + x[0].hi();
+  } else {
+#pragma unroll
+    for (int j = 0; j < V::P; ++j) *reinterpret_cast<float2 *>(tab + threadIdx.x * PER + 2 * j) = make_float2(x[j].lo(), x[j].hi());
+  }
+  __syncthreads();
+  // columns over pixel lanes, `split` threads per column where there are few
+  for (int i = threadIdx.x; i < split * width; i += THREADS) {
+    const int part = split == 1 ? 0 : small_div(i, a.inv_width), col = i - part * width;
     float s = 0.0f;
-    const int total = group_width * lanes;
-    for (int e = threadIdx.x & 31; e < total; e += 32) {
-      const int p = e / group_width;
-      s += tab[p * width + g * group_width + (e - p * group_width)];
-    }
+    for (int p = part; p < t.lanes; p += split) s += tab[p * width + col];
+    cols[i] = s;
+  }
+  __syncthreads();
+  // groups over columns, a warp each
+  const int group_width = ALIGNED ? a.cg / V::N : a.cg;
+  for (int g = threadIdx.x >> 5; g < t.n_groups; g += THREADS / 32) {
+    float s = 0.0f;
+    for (int e = threadIdx.x & 31; e < group_width; e += 32)
+      for (int k = 0; k < split; ++k) s += cols[k * width + g * group_width + e];
     s = warp_sum(s);
     if ((threadIdx.x & 31) == 0) done(g, s);
   }
 }
+// Calls use(j, group of channel ch + j, of the image) for the channels of a vector, behind the last group the last one.
+template <int N, class Use> __device__ __forceinline__ void for_groups(const GroupNormArgs &a, int ch, Use use) {
+  int g = small_div(ch, a.inv_cg), left = (g + 1) * a.cg - ch;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    use(j, min(g, a.groups - 1));
+    if (--left == 0) {
+      ++g;
+      left = a.cg;
+    }
+  }
+}
+// minus the mean of each channel's group; mean(group of the chunk)
+template <typename T, bool ALIGNED, class Mean>
+__device__ __forceinline__ void own_means(const GroupNormArgs &a, int ch, int first_group, int n_groups, Mean mean, Pair *m) {
+  if (ALIGNED) {
+    m[0] = both(-mean(min(small_div(ch, a.inv_cg) - first_group, n_groups - 1)));
+  } else {
+    float v[NormVec<T>::N];
+    for_groups<NormVec<T>::N>(a, ch, [&](int j, int g) { v[j] = -mean(min(g - first_group, n_groups - 1)); });
+#pragma unroll
+    for (int j = 0; j < NormVec<T>::P; ++j) m[j] = Pair(v[2 * j], v[2 * j + 1]);
+  }
+}
+// y = x scale + shift of a thread's channels
+template <typename T> struct NormAffine {
+  typedef NormVec<T> V;
+  Pair scale[V::P], shift[V::P];
+  __device__ __forceinline__ void load(const GroupNormArgs &a, int ch) {
+    load_floats(a.gamma + ch, scale);
+    load_floats(a.beta + ch, shift);
+  }
+  // `stat(group of the image)`: mean and 1 / sqrt(var + eps)
+  template <bool ALIGNED, class Stat> __device__ __forceinline__ void set(const GroupNormArgs &a, int ch, Stat stat) {
+    if (ALIGNED) {
+      const float2 st = stat(small_div(ch, a.inv_cg));
+#pragma unroll
+      for (int j = 0; j < V::P; ++j) {
+        scale[j] = scale[j] * both(st.y);
+        shift[j] = fma(both(-st.x), scale[j], shift[j]);
+      }
+    } else {
+      float2 st[V::N];
+      for_groups<V::N>(a, ch, [&](int j, int g) { st[j] = stat(g); });
+#pragma unroll
+      for (int j = 0; j < V::P; ++j) {
+        scale[j] = scale[j] * Pair(st[2 * j].y, st[2 * j + 1].y);
+        shift[j] = fma(Pair(-st[2 * j].x, -st[2 * j + 1].x), scale[j], shift[j]);
+      }
+    }
+  }
+  __device__ __forceinline__ uint4 apply(const GroupNormArgs &a, const uint4 &raw, int valid) const {
+    Pair x[V::P];
+    V::get(raw, x);
+#pragma unroll
+    for (int j = 0; j < V::P; ++j) x[j] = fma(x[j], scale[j], shift[j]);
+    activate_all<V::kF32>(a.act, x);
+    if (valid < V::N) clip(x, valid);
+    return V::put(x);
+  }
+};
 
 // ---- slab. ALIGNED: a vector's channels belong to one group. NV: vectors per thread.
-template <typename T, bool ALIGNED, int NV> __global__ void __launch_bounds__(kNormThreads) group_norm_slab_kernel(const GroupNormArgs a) {
+template <typename T, bool ALIGNED, int NV> __global__ void __launch_bounds__(kSlabThreads, NV <= 4 ? 2 : 1) group_norm_slab_kernel(const GroupNormArgs a) {
   typedef NormVec<T> V;
-  constexpr int PER = ALIGNED ? 1 : V::N;
   extern __shared__ float smem[];
-  float *tab = smem;                                                       // [threads][PER]
-  float2 *own = reinterpret_cast<float2 *>(smem + kNormThreads * PER);     // [groups of the chunk]: this block's mean and M2
-  float2 *all = own + a.chunk_groups;                                      // mean and 1 / sqrt(var + eps) of the image
-  const NormTile<T> t(a, blockIdx.x);
-  float ga[V::N], be[V::N];
-  int grp[PER];
-#pragma unroll
-  for (int j = 0; j < PER; ++j) grp[j] = min((t.ch + j) / a.cg - t.first_group, t.n_groups - 1); // (padded channels: any group)
-  if (t.active) {
-    load_floats(a.gamma + t.ch, ga);
-    load_floats(a.beta + t.ch, be);
-  }
+  float2 *own = reinterpret_cast<float2 *>(smem); // [groups of the chunk]: this block's mean and M2
+  float2 *all = own + a.chunk_groups;             // mean and 1 / sqrt(var + eps) of the image
+  float *tab = reinterpret_cast<float *>(all + a.chunk_groups);
+  const NormTile<T, kSlabThreads> t(a, blockIdx.x, a.parts, a.part_pixels);
+  constexpr int P = ALIGNED ? 1 : V::P;
+  const size_t at = t.offset(a, t.px0 + t.p), step = (size_t)t.lanes * a.cp;
+  const int mine = t.active ? t.px1 - t.px0 - t.p : 0; // pixels from the thread's first on
   pdl_prologue();
   const T *in = (const T *)a.in;
   uint4 raw[NV];
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int px = t.px0 + t.p + k * t.lanes;
-    if (t.active && px < t.px1) raw[k] = *reinterpret_cast<const uint4 *>(in + t.offset(a, px));
-  }
-  const int group_width = ALIGNED ? a.cg / V::N : a.cg;
-  const float count = (float)(t.px1 - t.px0) * (float)a.cg;
-  float acc[PER];
+  for (int k = 0; k < NV; ++k)
+    if (k * t.lanes < mine) raw[k] = *reinterpret_cast<const uint4 *>(in + at + k * step);
+  Pair sum[P];
 #pragma unroll
-  for (int j = 0; j < PER; ++j) acc[j] = 0.0f;
+  for (int j = 0; j < P; ++j) sum[j] = both(0.0f);
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    if (!(t.active && t.px0 + t.p + k * t.lanes < t.px1)) continue;
-    float x[V::N];
-    V::get(raw[k], x);
+  for (int k = 0; k < NV; ++k)
+    if (k * t.lanes < mine) {
+      Pair x[V::P];
+      V::get(raw[k], x);
 #pragma unroll
-    for (int j = 0; j < V::N; ++j) acc[ALIGNED ? 0 : j] += x[j];
-  }
-#pragma unroll
-  for (int j = 0; j < PER; ++j) tab[threadIdx.x * PER + j] = acc[j];
-  __syncthreads();
-  group_sums<PER>(tab, a.vecs, t.lanes, group_width, t.n_groups, [&](int g, float s) { own[g].x = s / count; });
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < PER; ++j) acc[j] = 0.0f;
-  float m[PER];
-#pragma unroll
-  for (int j = 0; j < PER; ++j) m[j] = own[grp[j]].x;
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    if (!(t.active && t.px0 + t.p + k * t.lanes < t.px1)) continue;
-    float x[V::N];
-    V::get(raw[k], x);
-#pragma unroll
-    for (int j = 0; j < V::N; ++j) {
-      const float d = x[j] - m[ALIGNED ? 0 : j];
-      acc[ALIGNED ? 0 : j] = fmaf(d, d, acc[ALIGNED ? 0 : j]);
+      for (int j = 0; j < V::P; ++j) sum[ALIGNED ? 0 : j] = sum[ALIGNED ? 0 : j] + x[j];
     }
-  }
-#pragma unroll
-  for (int j = 0; j < PER; ++j) tab[threadIdx.x * PER + j] = acc[j];
+  const float inv_count = 1.0f / ((float)(t.px1 - t.px0) * (float)a.cg);
+  norm_group_sums<T, ALIGNED, kSlabThreads>(a, t, sum, tab, [&](int g, float s) { own[g].x = s * inv_count; });
   __syncthreads();
-  group_sums<PER>(tab, a.vecs, t.lanes, group_width, t.n_groups, [&](int g, float s) { own[g].y = s; });
+  Pair mean_of[P]; // negative
+  own_means<T, ALIGNED>(a, t.ch, t.first_group, t.n_groups, [&](int g) { return own[g].x; }, mean_of);
+#pragma unroll
+  for (int j = 0; j < P; ++j) sum[j] = both(0.0f);
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+    if (k * t.lanes < mine) {
+      Pair x[V::P];
+      V::get(raw[k], x);
+#pragma unroll
+      for (int j = 0; j < V::P; ++j) {
+        const Pair d = x[j] + mean_of[ALIGNED ? 0 : j];
+        sum[ALIGNED ? 0 : j] = fma(d, d, sum[ALIGNED ? 0 : j]);
+      }
+    }
+  norm_group_sums<T, ALIGNED, kSlabThreads>(a, t, sum, tab, [&](int g, float s) { own[g].y = s; });
+  NormAffine<T> affine;
+  if (t.active) affine.load(a, t.ch);
   if (a.parts > 1) ptx::cluster_sync();
   else __syncthreads();
   const float total = (float)a.pixels * (float)a.cg;
-  for (int g = threadIdx.x; g < t.n_groups; g += kNormThreads) {
+  for (int g = threadIdx.x; g < t.n_groups; g += kSlabThreads) {
     float mean = own[g].x, m2 = own[g].y;
     if (a.parts > 1) {
-      float2 other[8];
-#pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        if (r >= a.parts) break;
+      auto pixels_of = [&](int r) { return (float)(min((r + 1) * a.part_pixels, a.pixels) - r * a.part_pixels); };
+      auto other = [&](int r) {
+        float2 o;
         const uint32_t at = ptx::map_cluster(ptx::smem_u32(&own[g]), (uint32_t)r);
-        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(other[r].x), "=f"(other[r].y) : "r"(at) : "memory");
-      }
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(o.x), "=f"(o.y) : "r"(at) : "memory");
+        return o;
+      };
       mean = m2 = 0.0f;
-#pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        if (r >= a.parts) break;
-        mean += other[r].x * ((float)(min((r + 1) * a.part_pixels, a.pixels) - r * a.part_pixels) / (float)a.pixels);
-      }
-#pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        if (r >= a.parts) break;
-        const float d = other[r].x - mean, n = (float)(min((r + 1) * a.part_pixels, a.pixels) - r * a.part_pixels) * (float)a.cg;
-        m2 += fmaf(d * d, n, other[r].y);
+#pragma unroll 1
+      for (int r = 0; r < a.parts; ++r) mean += other(r).x * (pixels_of(r) / (float)a.pixels);
+#pragma unroll 1
+      for (int r = 0; r < a.parts; ++r) {
+        const float2 o = other(r);
+        m2 += fmaf((o.x - mean) * (o.x - mean), pixels_of(r) * (float)a.cg, o.y);
       }
     }
     all[g] = make_float2(mean, rsqrtf(m2 / total + a.eps));
   }
   __syncthreads();
   if (a.parts > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); // the others' numbers have been read
-  float r[PER];
+  if (t.active) {
+    affine.template set<ALIGNED>(a, t.ch, [&](int g) { return all[g - t.first_group]; });
+    T *out = (T *)a.out;
 #pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    m[j] = all[grp[j]].x;
-    r[j] = all[grp[j]].y;
+    for (int k = 0; k < NV; ++k)
+      if (k * t.lanes < mine) *reinterpret_cast<uint4 *>(out + at + k * step) = affine.apply(a, raw[k], ALIGNED ? V::N : a.c - t.ch);
   }
-  T *out = (T *)a.out;
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int px = t.px0 + t.p + k * t.lanes;
-    if (!(t.active && px < t.px1)) continue;
-    float x[V::N];
-    V::get(raw[k], x);
-#pragma unroll
-    for (int j = 0; j < V::N; ++j) x[j] = fmaf((x[j] - m[ALIGNED ? 0 : j]) * r[ALIGNED ? 0 : j], ga[j], be[j]);
-    activate_all<V::kF32>(a.act, x);
-    if (!ALIGNED) {
-#pragma unroll
-      for (int j = 0; j < V::N; ++j) x[j] = t.ch + j < a.c ? x[j] : 0.0f;
-    }
-    *reinterpret_cast<uint4 *>(out + t.offset(a, px)) = V::put(x);
-  }
+  __syncwarp();
   if (a.parts > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); // none leaves while its numbers may be read
 }
 
 // ---- streamed
-template <typename T, bool ALIGNED> __global__ void __launch_bounds__(kNormThreads) group_norm_stats_kernel(const GroupNormArgs a) {
-  typedef NormVec<T> V;
-  constexpr int PER = ALIGNED ? 1 : V::N;
+template <typename T, bool ALIGNED> __global__ void __launch_bounds__(kStreamThreads, 2) group_norm_stats_kernel(const GroupNormArgs a) {
   extern __shared__ float smem[];
-  float *tab = smem;                                                   // [threads][PER]
-  float *mean_of = smem + kNormThreads * PER;                          // [groups of the chunk]
-  __shared__ int last;
-  const NormTile<T> t(a, blockIdx.x);
+  typedef NormVec<T> V;
+  constexpr int P = ALIGNED ? 1 : V::P;
+  const NormTile<T, kStreamThreads> t(a, blockIdx.x, a.parts, a.part_pixels);
+  float *mean_of = smem; // [groups of the chunk]
+  float *tab = smem + (a.chunk_groups + 1) / 2 * 2;
   pdl_prologue();
-  const T *in = (const T *)a.in;
-  const int mine = t.active && t.px0 + t.p < t.px1 ? (t.px1 - t.px0 - t.p + t.lanes - 1) / t.lanes : 0;
-  // Distances from the first value of each channel (or, where vectors lie within groups, of the vector)
-  float first[PER], s[PER], q[PER];
+  const int mine = t.active && t.px0 + t.p < t.px1 ? small_div(t.px1 - t.px0 - t.p + t.lanes - 1, a.inv_lanes) : 0;
+  Pair first[P], s[P], q[P]; // first: negative
 #pragma unroll
-  for (int j = 0; j < PER; ++j) first[j] = s[j] = q[j] = 0.0f;
-  const T *at = in + t.offset(a, t.px0 + t.p);
-  const size_t step = (size_t)t.lanes * a.cp;
+  for (int j = 0; j < P; ++j) first[j] = s[j] = q[j] = both(0.0f);
   auto take = [&](const uint4 &raw) {
-    float x[V::N];
+    Pair x[V::P];
     V::get(raw, x);
 #pragma unroll
-    for (int j = 0; j < V::N; ++j) {
+    for (int j = 0; j < V::P; ++j) {
       const int i = ALIGNED ? 0 : j;
-      const float d = x[j] - first[i];
-      s[i] += d;
-      q[i] = fmaf(d, d, q[i]);
+      const Pair d = x[j] + first[i];
+      s[i] = s[i] + d;
+      q[i] = fma(d, d, q[i]);
     }
   };
   if (mine > 0) {
-    float x[V::N];
-    V::get(*reinterpret_cast<const uint4 *>(at), x);
+    const T *at = (const T *)a.in + t.offset(a, t.px0 + t.p);
+    const size_t step = (size_t)t.lanes * a.cp;
+    {
+      Pair x[V::P];
+      V::get(*reinterpret_cast<const uint4 *>(at), x);
 #pragma unroll
-    for (int j = 0; j < PER; ++j) first[j] = x[j];
-  }
-  int k = 0;
-  for (; k + 8 <= mine; k += 8) {
-    uint4 raw[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) raw[i] = *reinterpret_cast<const uint4 *>(at + i * step);
-    at += 8 * step;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) take(raw[i]);
-  }
-  for (; k < mine; ++k, at += step) take(*reinterpret_cast<const uint4 *>(at));
-  // per thread: count n, mean = first + s / n, M2 = q - s^2 / n
-  const float n = (float)mine * (ALIGNED ? V::N : 1);
-  const int group_width = ALIGNED ? a.cg / V::N : a.cg;
-  const float count = (float)(t.px1 - t.px0) * (float)a.cg;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    if (mine > 0) {
-      q[j] -= s[j] * (s[j] / n);
-      q[j] = q[j] < 0.0f ? 0.0f : q[j]; // (a NaN stays)
-      first[j] += s[j] / n;
+      for (int j = 0; j < P; ++j) first[j] = ALIGNED ? both(-x[0].lo()) : x[j] * both(-1.0f);
     }
-    tab[threadIdx.x * PER + j] = n * first[j];
-  }
-  __syncthreads();
-  group_sums<PER>(tab, a.vecs, t.lanes, group_width, t.n_groups, [&](int g, float v) { mean_of[g] = v / count; });
-  __syncthreads();
+    int k = 0;
+    for (; k + 4 <= mine; k += 4) {
+      uint4 raw[4];
 #pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const float d = first[j] - mean_of[min((t.ch + j) / a.cg - t.first_group, t.n_groups - 1)];
-    tab[threadIdx.x * PER + j] = mine > 0 ? fmaf(n * d, d, q[j]) : 0.0f;
+      for (int i = 0; i < 4; ++i) raw[i] = *reinterpret_cast<const uint4 *>(at + i * step);
+      at += 4 * step;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) take(raw[i]);
+    }
+    for (; k < mine; ++k, at += step) take(*reinterpret_cast<const uint4 *>(at));
   }
+  // The thread's count, mean and M2 (per channel; where vectors lie within groups both halves count as columns of their own)
+  const float n = (float)mine * (ALIGNED ? V::P : 1), inv = mine > 0 ? 1.0f / n : 0.0f;
+  const float inv_count = 1.0f / ((float)(t.px1 - t.px0) * (float)a.cg);
+  Pair x[P];
+#pragma unroll
+  for (int j = 0; j < P; ++j) {
+    const Pair mean = s[j] * both(inv);
+    q[j] = fma(s[j] * both(-1.0f), mean, q[j]);
+    q[j] = Pair(q[j].lo() < 0.0f ? 0.0f : q[j].lo(), q[j].hi() < 0.0f ? 0.0f : q[j].hi()); // (a NaN stays)
+    first[j] = fma(first[j], both(-1.0f), mean); // the mean
+    x[j] = first[j] * both(n);
+  }
+  norm_group_sums<T, ALIGNED, kStreamThreads>(a, t, x, tab, [&](int g, float sum) { mean_of[g] = sum * inv_count; });
   __syncthreads();
+  Pair m[P];
+  own_means<T, ALIGNED>(a, t.ch, t.first_group, t.n_groups, [&](int g) { return mean_of[g]; }, m);
+#pragma unroll
+  for (int j = 0; j < P; ++j) {
+    const Pair d = first[j] + m[j];
+    x[j] = mine > 0 ? fma(d * both(n), d, q[j]) : both(0.0f);
+  }
   float2 *partial = a.partial + ((size_t)t.img * a.groups + t.first_group) * a.parts;
-  group_sums<PER>(tab, a.vecs, t.lanes, group_width, t.n_groups,
-                  [&](int g, float v) { partial[(size_t)g * a.parts + t.part] = make_float2(mean_of[g], v); });
-  // the block that comes last joins the parts, in their order
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) last = atomicAdd(a.arrived + t.img * a.chunks + t.chunk, 1u) == (unsigned)a.parts - 1;
-  __syncthreads();
-  if (!last) return;
-  __threadfence();
-  for (int g = threadIdx.x >> 5; g < t.n_groups; g += kNormThreads / 32) {
-    const volatile float2 *pp = partial + (size_t)g * a.parts;
-    auto share = [&](int r) { return (float)(min((r + 1) * a.part_pixels, a.pixels) - r * a.part_pixels); };
-    float mean = 0.0f, m2 = 0.0f;
-    for (int r = threadIdx.x & 31; r < a.parts; r += 32) mean += pp[r].x * (share(r) / (float)a.pixels);
-    mean = warp_sum(mean);
-    for (int r = threadIdx.x & 31; r < a.parts; r += 32) {
-      const float d = pp[r].x - mean;
-      m2 += fmaf(d * d, share(r) * (float)a.cg, pp[r].y);
-    }
-    m2 = warp_sum(m2);
-    if ((threadIdx.x & 31) == 0)
-      a.stats[(size_t)t.img * a.groups + t.first_group + g] = make_float2(mean, rsqrtf(m2 / ((float)a.pixels * (float)a.cg) + a.eps));
-  }
-  if (threadIdx.x == 0) a.arrived[t.img * a.chunks + t.chunk] = 0u;
+  norm_group_sums<T, ALIGNED, kStreamThreads>(a, t, x, tab, [&](int g, float sum) { partial[(size_t)g * a.parts + t.part] = make_float2(mean_of[g], sum); });
 }
 
-template <typename T> __global__ void __launch_bounds__(kNormThreads) group_norm_apply_kernel(const GroupNormArgs a) {
-  typedef NormVec<T> V;
-  const NormTile<T> t(a, gridDim.x - 1 - blockIdx.x);
-  float sc[V::N], be[V::N], m[V::N];
-  if (t.active) {
-    load_floats(a.gamma + t.ch, sc);
-    load_floats(a.beta + t.ch, be);
-  }
+template <typename T, bool ALIGNED> __global__ void __launch_bounds__(kStreamThreads, 2) group_norm_apply_kernel(const GroupNormArgs a) {
+  extern __shared__ float smem[];
+  float2 *stats = reinterpret_cast<float2 *>(smem); // [groups of the chunk]: mean, 1 / sqrt(var + eps)
+  const NormTile<T, kStreamThreads> t(a, gridDim.x - 1 - blockIdx.x, a.apply_parts, a.apply_pixels);
+  NormAffine<T> affine;
+  if (t.active) affine.load(a, t.ch);
   pdl_prologue();
-  if (!t.active) return;
-#pragma unroll
-  for (int j = 0; j < V::N; ++j) {
-    const float2 st = a.stats[(size_t)t.img * a.groups + min((t.ch + j) / a.cg, a.groups - 1)];
-    m[j] = st.x;
-    sc[j] *= st.y;
+  // the parts, in their order: a warp per group
+  const float inv_pixels = 1.0f / (float)a.pixels, cg = (float)a.cg;
+  auto share = [&](int r) { return (float)(min((r + 1) * a.part_pixels, a.pixels) - r * a.part_pixels); };
+  for (int g = threadIdx.x >> 5; g < t.n_groups; g += kStreamThreads / 32) {
+    const float2 *partial = a.partial + ((size_t)t.img * a.groups + t.first_group + g) * a.parts;
+    const int lane = threadIdx.x & 31;
+    float mean = 0.0f, m2 = 0.0f;
+#pragma unroll 4
+    for (int r = lane; r < a.parts; r += 32) mean += partial[r].x * (share(r) * inv_pixels);
+    mean = warp_sum(mean);
+#pragma unroll 4
+    for (int r = lane; r < a.parts; r += 32) {
+      const float2 o = partial[r];
+      m2 += fmaf((o.x - mean) * (o.x - mean), share(r) * cg, o.y);
+    }
+    m2 = warp_sum(m2);
+    if (lane == 0) stats[g] = make_float2(mean, rsqrtf(m2 * inv_pixels / cg + a.eps));
   }
-  const int mine = t.px0 + t.p < t.px1 ? (t.px1 - t.px0 - t.p + t.lanes - 1) / t.lanes : 0;
+  __syncthreads();
+  if (!t.active) return;
+  affine.template set<ALIGNED>(a, t.ch, [&](int g) { return stats[g - t.first_group]; });
+  const int mine = t.px0 + t.p < t.px1 ? small_div(t.px1 - t.px0 - t.p + t.lanes - 1, a.inv_lanes) : 0, valid = ALIGNED ? NormVec<T>::N : a.c - t.ch;
   const size_t step = (size_t)t.lanes * a.cp;
   // from the last pixel to the first
   size_t at = t.offset(a, t.px0 + t.p) + (size_t)max(mine - 1, 0) * step;
   const T *in = (const T *)a.in;
   T *out = (T *)a.out;
-  auto put = [&](const uint4 &raw, size_t o) {
-    float x[V::N];
-    V::get(raw, x);
-#pragma unroll
-    for (int j = 0; j < V::N; ++j) x[j] = fmaf(x[j] - m[j], sc[j], be[j]);
-    activate_all<V::kF32>(a.act, x);
-#pragma unroll
-    for (int j = 0; j < V::N; ++j) x[j] = t.ch + j < a.c ? x[j] : 0.0f;
-    *reinterpret_cast<uint4 *>(out + o) = V::put(x);
-  };
   int k = 0;
   for (; k + 4 <= mine; k += 4) {
     uint4 raw[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) raw[i] = *reinterpret_cast<const uint4 *>(in + at - i * step);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) put(raw[i], at - i * step);
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4 *>(out + at - i * step) = affine.apply(a, raw[i], valid);
     at -= 4 * step;
   }
-  for (; k < mine; ++k, at -= step) put(*reinterpret_cast<const uint4 *>(in + at), at);
+  for (; k < mine; ++k, at -= step) *reinterpret_cast<uint4 *>(out + at) = affine.apply(a, *reinterpret_cast<const uint4 *>(in + at), valid);
 }
 
 // ---- strided: one block per image and group, three passes over its values
@@ -502,45 +518,48 @@ template <typename T> __global__ void group_norm_strided_kernel(const GroupNormA
   for (size_t i = threadIdx.x; i < count; i += blockDim.x) {
     const size_t o = at(i);
     const int ch = g * a.cg + (int)(o % a.cp);
-    float v[1] = {fmaf((V::one(in[o]) - mean) * rstd, a.gamma[ch], a.beta[ch])};
+    Pair v[1] = {both(fmaf((V::one(in[o]) - mean) * rstd, a.gamma[ch], a.beta[ch]))};
     activate_all<V::kF32>(a.act, v);
-    out[o] = V::back(v[0]);
+    out[o] = V::back(v[0].lo());
   }
 }
 
 inline void launch_group_norm(const GroupNormArgs &a, const GroupNormPlan &p, bool f32, cudaStream_t s) {
   auto by_type = [&](auto type) {
     typedef decltype(type) T;
-    auto by_nv = [&](auto nv) {
+    auto rows = [&](auto nv, auto block) {
       constexpr int NV = decltype(nv)::value;
-      if (p.form == NORM_ROWS_WARP) launch_k(group_norm_rows_kernel<T, NV, false>, p.grid, 128, 0, s, a);
-      else if constexpr (NV <= 4) launch_k(group_norm_rows_kernel<T, NV, true>, p.grid, p.threads, 0, s, a);
+      constexpr bool BLOCK = decltype(block)::value;
+      if (a.cg % NormVec<T>::N) launch_k(group_norm_rows_kernel<T, NV, BLOCK, true>, p.grid, p.threads, 0, s, a);
+      else launch_k(group_norm_rows_kernel<T, NV, BLOCK, false>, p.grid, p.threads, 0, s, a);
     };
-    auto slab_nv = [&](auto nv) {
+    auto slab = [&](auto nv) {
       constexpr int NV = decltype(nv)::value;
-      if (p.aligned) launch_cluster_k(a.parts, group_norm_slab_kernel<T, true, NV>, p.grid, kNormThreads, p.smem, s, a);
-      else launch_cluster_k(a.parts, group_norm_slab_kernel<T, false, NV>, p.grid, kNormThreads, p.smem, s, a);
+      if (p.aligned) launch_cluster_k(a.parts, group_norm_slab_kernel<T, true, NV>, dim3(p.grid, a.chunks), p.threads, p.smem, s, a);
+      else launch_cluster_k(a.parts, group_norm_slab_kernel<T, false, NV>, dim3(p.grid, a.chunks), p.threads, p.smem, s, a);
+    };
+    auto by_nv = [&](auto use) {
+      if (p.nv <= 1) use(std::integral_constant<int, 1>());
+      else if (p.nv <= 2) use(std::integral_constant<int, 2>());
+      else if (p.nv <= 4) use(std::integral_constant<int, 4>());
+      else use(std::integral_constant<int, 8>());
     };
     switch (p.form) {
-    case NORM_ROWS_WARP:
-    case NORM_ROWS_BLOCK:
-      if (p.nv <= 1) by_nv(std::integral_constant<int, 1>());
-      else if (p.nv <= 2) by_nv(std::integral_constant<int, 2>());
-      else if (p.nv <= 4) by_nv(std::integral_constant<int, 4>());
-      else by_nv(std::integral_constant<int, 8>());
+    case NORM_ROWS_WARP: by_nv([&](auto nv) { rows(nv, std::false_type()); }); break;
+    case NORM_ROWS_BLOCK: by_nv([&](auto nv) { rows(nv, std::true_type()); }); break;
+    case NORM_SLAB: by_nv(slab); break;
+    case NORM_STREAMED: {
+      auto both_passes = [&](auto aligned) {
+        constexpr bool A = decltype(aligned)::value;
+        launch_k(group_norm_stats_kernel<T, A>, dim3(p.grid, a.chunks), p.threads, p.smem, s, a);
+        PdlConvScope overlap; // the second pass fetches gamma and beta while the first ends
+        launch_k(group_norm_apply_kernel<T, A>, dim3(p.apply_grid, a.chunks), p.threads, (size_t)a.chunk_groups * sizeof(float2), s, a);
+      };
+      if (p.aligned) both_passes(std::true_type());
+      else both_passes(std::false_type());
       break;
-    case NORM_SLAB:
-      if (p.nv <= 2) slab_nv(std::integral_constant<int, 2>());
-      else if (p.nv <= 4) slab_nv(std::integral_constant<int, 4>());
-      else if (p.nv <= 8) slab_nv(std::integral_constant<int, 8>());
-      else slab_nv(std::integral_constant<int, 16>());
-      break;
-    case NORM_STREAMED:
-      if (p.aligned) launch_k(group_norm_stats_kernel<T, true>, p.grid, kNormThreads, p.smem, s, a);
-      else launch_k(group_norm_stats_kernel<T, false>, p.grid, kNormThreads, p.smem, s, a);
-      launch_k(group_norm_apply_kernel<T>, p.grid, kNormThreads, 0, s, a);
-      break;
-    default: launch_k(group_norm_strided_kernel<T>, p.grid, kNormThreads, 0, s, a);
+    }
+    default: launch_k(group_norm_strided_kernel<T>, p.grid, p.threads, 0, s, a);
     }
   };
   if (f32) by_type(float());

@@ -1961,13 +1961,15 @@ public:
     a_.gamma = I.upload(s.gamma); a_.beta = I.upload(s.beta);
     a_.n = in->n; a_.pixels = in->h * in->w; a_.c = in->c; a_.cp = in->cp; a_.groups = s.groups; a_.cg = in->c / s.groups;
     a_.eps = s.eps; a_.act = s.act;
+    const int columns = plan_.vecs * (plan_.aligned ? 1 : 16 / (int)in->elsize());
+    a_.lanes = plan_.lanes;
+    a_.col_split = std::max(1, (int)plan_.threads / columns);
+    a_.inv_vecs = 1.0f / plan_.vecs; a_.inv_lanes = 1.0f / plan_.lanes; a_.inv_cg = 1.0f / a_.cg; a_.inv_width = 1.0f / columns;
     a_.vecs = plan_.vecs; a_.chunk_groups = plan_.chunk_groups; a_.chunks = plan_.chunks; a_.parts = plan_.parts; a_.part_pixels = plan_.part_pixels;
     if (plan_.form == NORM_STREAMED) {
-      const size_t rows = (size_t)in->n * s.groups, counters = (size_t)in->n * plan_.chunks;
-      a_.partial = (float2 *)I.dalloc(rows * plan_.parts * sizeof(float2));
-      a_.stats = (float2 *)I.dalloc(rows * sizeof(float2));
-      a_.arrived = (unsigned *)I.dalloc(counters * sizeof(unsigned));
-      TPUCB_CUDA(cudaMemsetAsync(a_.arrived, 0, counters * sizeof(unsigned), I.stream));
+      a_.apply_parts = plan_.apply_parts;
+      a_.apply_pixels = plan_.apply_pixels;
+      a_.partial = (float2 *)I.dalloc((size_t)in->n * s.groups * plan_.parts * sizeof(float2));
     }
     alg_ops = 8.0 * in->numel();
     alg_bytes = 2.0 * in->numel() * in->elsize() + 8.0 * in->c;

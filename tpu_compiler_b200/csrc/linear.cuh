@@ -45,7 +45,7 @@ template <typename T, int ACT> __global__ void __launch_bounds__(256) linear_ker
       const int ch = n0 + tx * 4 + j;
       if (ch >= a.n) break;
       const size_t o = (size_t)row * a.ldy + ch;
-      float v = activate<ACT, F32>(acc[i][j] + a.bias[ch]);
+      float v = activate<ACT, F32>(both(acc[i][j] + a.bias[ch])).lo();
       if (a.res) v += get(a.res, o);
       if (F32) ((float *)a.y)[o] = v;
       else ((uint16_t *)a.y)[o] = (uint16_t)bf16x2_ieee(v, v);

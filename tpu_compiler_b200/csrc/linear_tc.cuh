@@ -66,18 +66,13 @@ template <int ACT> __device__ __forceinline__ void linear_finish16(const float *
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const float4 b = __ldg(bias + q);
-    float v[4] = {acc[4 * q] + b.x, acc[4 * q + 1] + b.y, acc[4 * q + 2] + b.z, acc[4 * q + 3] + b.w};
+    Pair v[2] = {activate<ACT, false>(Pair(acc[4 * q], acc[4 * q + 1]) + Pair(b.x, b.y)),
+                 activate<ACT, false>(Pair(acc[4 * q + 2], acc[4 * q + 3]) + Pair(b.z, b.w))};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = activate<ACT, false>(v[j]);
-    if (p.res) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        v[2 * j] += __uint_as_float(r[2 * q + j] << 16);
-        v[2 * j + 1] += __uint_as_float(r[2 * q + j] & 0xffff0000u);
-      }
+    for (int j = 0; j < 2; ++j) {
+      if (p.res) v[j] = v[j] + pair_of_bf16(r[2 * q + j]);
+      o[2 * q + j] = bf16x2_ieee(v[j].lo(), v[j].hi());
     }
-    o[2 * q] = bf16x2_ieee(v[0], v[1]);
-    o[2 * q + 1] = bf16x2_ieee(v[2], v[3]);
   }
   ptx::st_global_32b(p.y + at, o);
 }

@@ -99,12 +99,15 @@ inline LinearSpec linear_spec(const ParsedOp &op, const DevTensor &in, const Dev
 
 // ---- how a group norm runs (group_norm.cuh)
 enum NormForm { NORM_ROWS_WARP = 0, NORM_ROWS_BLOCK, NORM_SLAB, NORM_STREAMED, NORM_STRIDED };
+constexpr int kSlabThreads = 512, kStreamThreads = 512;
 struct GroupNormPlan {
   int form = NORM_STRIDED;
   unsigned grid = 0, threads = 256;
   int nv = 1;             // vectors per thread
   bool aligned = false;   // a vector's channels belong to one group
-  int vecs = 0, chunk_groups = 0, chunks = 0, parts = 1, part_pixels = 0;
+  int vecs = 1, lanes = 1, chunk_groups = 0, chunks = 0, parts = 1, part_pixels = 0;
+  int apply_parts = 1, apply_pixels = 0;
+  unsigned apply_grid = 0;
   size_t smem = 0;
 };
 // mode (option "norm_form"): 0 by size, else 1 + the form, where it can
@@ -115,59 +118,68 @@ inline GroupNormPlan group_norm_plan(int n, int pixels, int c, int groups, int e
   p.aligned = cg % N == 0;
   if (mode == 1 + NORM_STRIDED) return p;
   if (pixels == 1 && (p.aligned || groups == 1) && mode <= 1 + NORM_ROWS_BLOCK) {
-    // a warp keeps up to 8 vectors per lane, a block of up to 1024 threads 4
+    // a thread keeps up to 8 vectors: a warp 256, a block of up to 512 threads 4096
     const int nvec = (cg + N - 1) / N;
     if (nvec <= 8 * 32 && mode != 1 + NORM_ROWS_BLOCK) {
       p.form = NORM_ROWS_WARP;
       p.nv = (nvec + 31) / 32;
+      p.threads = 128;
       p.grid = (unsigned)(((long long)n * groups + 3) / 4);
       return p;
     }
-    if (nvec <= 4096) {
+    if (nvec <= 8 * 512) {
       p.form = NORM_ROWS_BLOCK;
-      p.threads = 32;
-      while ((int)p.threads * 4 < nvec) p.threads *= 2;
+      p.threads = 128;
+      while (p.threads < 512 && (int)p.threads * 4 < nvec) p.threads *= 2;
       p.nv = (nvec + p.threads - 1) / p.threads;
       return p;
     }
   }
   // chunks: whole groups and whole vectors; the smallest such unit, or the whole row
+  if (c >= 1 << 20 || (long long)n * 8 >= 1LL << 31) return p; // (small_div; the grid)
   int unit_groups = 1;
   while (unit_groups < groups && unit_groups * cg % N) ++unit_groups;
   const int unit_vecs = (unit_groups * cg + N - 1) / N;
   if (unit_vecs > 256) return p;
-  if (unit_groups * cg % N && unit_groups != groups) return p;
   const int units = (groups + unit_groups - 1) / unit_groups;
-  auto lay_out = [&](int k, int parts) { // k units per chunk
-    k = std::max(1, std::min(k, std::min(units, 256 / unit_vecs)));
+  auto lay_out = [&](int threads, int k, int parts) { // k units per chunk
+    k = std::max(1, std::min(k, std::min(units, threads / unit_vecs)));
     p.vecs = k * unit_vecs;
     p.chunk_groups = std::min(groups, k * unit_groups);
     p.chunks = (groups + p.chunk_groups - 1) / p.chunk_groups;
     p.part_pixels = (pixels + parts - 1) / parts;
     p.parts = (pixels + p.part_pixels - 1) / p.part_pixels;
-    const int lanes = 256 / p.vecs;
-    p.nv = (p.part_pixels + lanes - 1) / lanes;
-    p.grid = (unsigned)((long long)n * p.chunks * p.parts);
-    p.threads = 256;
+    const int per = p.aligned ? 1 : N;
+    p.lanes = threads / p.vecs;
+    p.nv = (p.part_pixels + p.lanes - 1) / p.lanes;
+    p.threads = (unsigned)threads;
+    p.grid = (unsigned)((long long)n * p.parts); // x chunks
+    p.smem = ((size_t)threads * per + std::max(threads, p.vecs * per) + round_up(p.chunk_groups, 2)) * 4;
   };
-  // slab: 64 bytes of a pixel and more, at most 16 vectors per thread in at most eight blocks
-  lay_out((4 + unit_vecs - 1) / unit_vecs, 1);
-  const int lanes = 256 / p.vecs, need = (pixels + 16 * lanes - 1) / (16 * lanes);
-  if (need <= 8 && mode != 1 + NORM_STREAMED) {
+  // slab: 64 bytes of a pixel and more, at most 8 vectors per thread in at most eight blocks
+  const int wide = (4 + unit_vecs - 1) / unit_vecs;
+  lay_out(kSlabThreads, wide, 1);
+  const int lanes = kSlabThreads / p.vecs, need = (pixels + 8 * lanes - 1) / (8 * lanes);
+  if (need <= 8 && mode != 1 + NORM_STREAMED && p.smem + (size_t)p.chunk_groups * 16 <= 48 * 1024) { // (shared memory that a kernel has unasked)
     int parts = need;
-    while (parts < 8 && (long long)n * p.chunks * parts * 2 <= 2 * sm_count && pixels > 2 * parts * lanes * 2) parts *= 2;
-    lay_out((4 + unit_vecs - 1) / unit_vecs, std::min(parts, 8));
+    while (parts < 8 && (long long)n * p.chunks * parts <= sm_count && pixels > 2 * parts * lanes) parts *= 2;
+    lay_out(kSlabThreads, wide, std::min(parts, 8));
     p.form = NORM_SLAB;
-    p.smem = (size_t)256 * (p.aligned ? 1 : N) * 4 + (size_t)p.chunk_groups * 16;
-    return p;
+    p.smem += (size_t)p.chunk_groups * 16;
+    // ... where its blocks all run at once
+    if (mode == 1 + NORM_SLAB || (long long)p.grid * p.chunks <= (p.nv <= 4 ? 2LL : 1LL) * sm_count) return p;
   }
-  // streamed: whole rows where they fit, four blocks' worth of work per SM
-  lay_out(1 << 20, 1);
-  const long long slabs = (long long)n * p.chunks;
-  const int most = (pixels + 256 / p.vecs - 1) / (256 / p.vecs); // parts of at least one vector per thread
-  lay_out(1 << 20, (int)std::max<long long>(1, std::min<long long>(most, (4LL * sm_count + slabs - 1) / slabs)));
+  // streamed: chunks of whole rows where they fit, and as many parts of the image as fill the SMs; a thread has 8 vectors at least
+  const int most_units = std::max(1, 256 / unit_vecs);
+  lay_out(kStreamThreads, most_units, 1);
+  const long long slabs = (long long)n * p.chunks, fill = std::max(1LL, sm_count / slabs), per_part = 8LL * p.lanes;
+  const int parts = (int)std::max(1LL, std::min(fill, (pixels + per_part - 1) / per_part));
+  const int apply = (int)std::max(1LL, std::min(2 * fill, (pixels + per_part - 1) / per_part));
+  lay_out(kStreamThreads, most_units, std::max(parts, (int)((pixels + (1LL << 22) - 1) >> 22))); // (small_div)
+  p.apply_pixels = (pixels + std::max(apply, p.parts) - 1) / std::max(apply, p.parts);
+  p.apply_parts = (pixels + p.apply_pixels - 1) / p.apply_pixels;
+  p.apply_grid = (unsigned)((long long)n * p.apply_parts);
   p.form = NORM_STREAMED;
-  p.smem = (size_t)256 * (p.aligned ? 1 : N) * 4 + (size_t)p.chunk_groups * 4;
   return p;
 }
 
