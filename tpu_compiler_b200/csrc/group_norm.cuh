@@ -33,8 +33,8 @@ struct GroupNormArgs {
   // slab and streamed: chunks of `vecs` vectors = whole groups (the last may have fewer), `parts` blocks share an image's pixels
   int vecs, lanes, chunk_groups, chunks, parts, part_pixels; // (lanes: pixels that a block's threads take at once)
   int apply_parts, apply_pixels; // streamed: of the second pass
-  int col_split;                 // norm_group_sums: threads per column, max(1, threads / columns)
-  float inv_vecs, inv_lanes, inv_cg, inv_width;        // 1 / vecs and so on, for quotients of small numbers (small_div)
+  int col_split, group_span;     // norm_group_sums: threads per column; parts of columns per group, rounded up to whole warps
+  float inv_vecs, inv_lanes, inv_cg, inv_width, inv_group_width;        // 1 / vecs and so on, for quotients of small numbers (small_div)
   float2 *partial;               // streamed: [n][groups][parts] mean, M2
 };
 // a / b for a < 2^22, given 1 / b: a + 1/2 is at least 1 / (2 b) of a quotient away from the next whole one, and the product's error less
@@ -166,7 +166,7 @@ template <typename T, int NV, bool BLOCK, bool TAIL> __global__ void __launch_bo
     load_floats(a.beta + g * a.cg + i * V::N, be);
     V::get(raw[k], x);
 #pragma unroll
-    for (int j = 0; j < V::P; ++j) x[j] = fma((x[j] + both(-mean)) * both(rstd), ga[j], be[j]);
+    for (int j = 0; j < V::P; ++j) x[j] = fma(fma(x[j], both(rstd), both(-mean * rstd)), ga[j], be[j]);
     activate_all<V::kF32>(a.act, x);
     if (TAIL && (i + 1) * V::N > a.cg) clip(x, a.cg - i * V::N);
     out[i] = V::put(x);
@@ -196,14 +196,16 @@ template <typename T, int THREADS> struct NormTile { // (parts: of the image, of
   __device__ __forceinline__ size_t offset(const GroupNormArgs &a, int px) const { return ((size_t)img * a.pixels + px) * a.cp + ch; }
 };
 // The block's sum over each group of its chunk of what the threads hold per channel or, where vectors lie within groups (ALIGNED), in
-// all: `done(group of the chunk, sum)` in lane 0 of a warp. tab: THREADS x PER floats, then max(THREADS, columns).
+// all: `done(group of the chunk, sum)` in one thread each. Three short steps, as these sums are what small tensors take their time for
+// (with a warp per group and a loop over all of its values, 2 x 1280 x 8 x 8 took 3.4 us instead of 2.2): columns (vectors or channels)
+// over the pixel lanes, several threads per column; warps over 32 of a group's column parts; groups over their warps' sums.
+// tab: THREADS x PER floats, then a.group_span per group, then that / 32; the parts behind a group's last are zero (norm_clear).
 template <typename T, bool ALIGNED, int THREADS, class Done>
 __device__ __forceinline__ void norm_group_sums(const GroupNormArgs &a, const NormTile<T, THREADS> &t, const Pair *x, float *tab, Done done) {
   typedef NormVec<T> V;
   constexpr int PER = ALIGNED ? 1 : V::N;
-  const int width = a.vecs * PER; // columns: vectors or channels
-  const int split = a.col_split; // threads per column
-  float *cols = tab + THREADS * PER;
+  const int width = a.vecs * PER, group_width = ALIGNED ? a.cg / V::N : a.cg;
+  float *cols = tab + THREADS * PER, *warps = cols + a.chunk_groups * a.group_span;
   if constexpr (ALIGNED) {
     tab[threadIdx.x] = x[0].lo() + x[0].hi();
   } else {
@@ -211,23 +213,31 @@ __device__ __forceinline__ void norm_group_sums(const GroupNormArgs &a, const No
     for (int j = 0; j < V::P; ++j) *reinterpret_cast<float2 *>(tab + threadIdx.x * PER + 2 * j) = make_float2(x[j].lo(), x[j].hi());
   }
   __syncthreads();
-  // columns over pixel lanes, `split` threads per column where there are few
-  for (int i = threadIdx.x; i < split * width; i += THREADS) {
-    const int part = split == 1 ? 0 : small_div(i, a.inv_width), col = i - part * width;
+  for (int i = threadIdx.x; i < a.col_split * width; i += THREADS) {
+    const int part = a.col_split == 1 ? 0 : small_div(i, a.inv_width), col = i - part * width, g = small_div(col, a.inv_group_width);
     float s = 0.0f;
-    for (int p = part; p < t.lanes; p += split) s += tab[p * width + col];
-    cols[i] = s;
+#pragma unroll 4
+    for (int p = part; p < t.lanes; p += a.col_split) s += tab[p * width + col];
+    if (g < t.n_groups) cols[g * a.group_span + part * group_width + col - g * group_width] = s;
   }
   __syncthreads();
-  // groups over columns, a warp each
-  const int group_width = ALIGNED ? a.cg / V::N : a.cg;
-  for (int g = threadIdx.x >> 5; g < t.n_groups; g += THREADS / 32) {
-    float s = 0.0f;
-    for (int e = threadIdx.x & 31; e < group_width; e += 32)
-      for (int k = 0; k < split; ++k) s += cols[k * width + g * group_width + e];
-    s = warp_sum(s);
-    if ((threadIdx.x & 31) == 0) done(g, s);
+  const int span = a.group_span >> 5; // warps' sums per group
+  for (int b = threadIdx.x >> 5; b < t.n_groups * span; b += THREADS / 32) {
+    const float s = warp_sum(cols[b * 32 + (threadIdx.x & 31)]);
+    if ((threadIdx.x & 31) == 0) warps[b] = s;
   }
+  __syncthreads();
+  for (int g = threadIdx.x; g < t.n_groups; g += THREADS) {
+    float s = 0.0f;
+#pragma unroll 4
+    for (int b = 0; b < span; ++b) s += warps[g * span + b];
+    done(g, s);
+  }
+}
+// before the first norm_group_sums (whose barriers order it)
+template <typename T, bool ALIGNED, int THREADS> __device__ __forceinline__ void norm_clear(const GroupNormArgs &a, float *tab) {
+  float *cols = tab + THREADS * (ALIGNED ? 1 : NormVec<T>::N);
+  for (int i = threadIdx.x; i < a.chunk_groups * a.group_span; i += THREADS) cols[i] = 0.0f;
 }
 // Calls use(j, group of channel ch + j, of the image) for the channels of a vector, behind the last group the last one.
 template <int N, class Use> __device__ __forceinline__ void for_groups(const GroupNormArgs &a, int ch, Use use) {
@@ -305,6 +315,7 @@ template <typename T, bool ALIGNED, int NV> __global__ void __launch_bounds__(kS
   pdl_prologue();
   const T *in = (const T *)a.in;
   uint4 raw[NV];
+  norm_clear<T, ALIGNED, kSlabThreads>(a, tab);
 #pragma unroll
   for (int k = 0; k < NV; ++k)
     if (k * t.lanes < mine) raw[k] = *reinterpret_cast<const uint4 *>(in + at + k * step);
@@ -385,6 +396,7 @@ template <typename T, bool ALIGNED> __global__ void __launch_bounds__(kStreamThr
   const NormTile<T, kStreamThreads> t(a, blockIdx.x, a.parts, a.part_pixels);
   float *mean_of = smem; // [groups of the chunk]
   float *tab = smem + (a.chunk_groups + 1) / 2 * 2;
+  norm_clear<T, ALIGNED, kStreamThreads>(a, tab);
   pdl_prologue();
   const int mine = t.active && t.px0 + t.p < t.px1 ? small_div(t.px1 - t.px0 - t.p + t.lanes - 1, a.inv_lanes) : 0;
   Pair first[P], s[P], q[P]; // first: negative
@@ -411,13 +423,14 @@ template <typename T, bool ALIGNED> __global__ void __launch_bounds__(kStreamThr
       for (int j = 0; j < P; ++j) first[j] = ALIGNED ? both(-x[0].lo()) : x[j] * both(-1.0f);
     }
     int k = 0;
-    for (; k + 4 <= mine; k += 4) {
-      uint4 raw[4];
+    constexpr int DEPTH = ALIGNED ? 8 : 4; // loads in flight, as the registers allow
+    for (; k + DEPTH <= mine; k += DEPTH) {
+      uint4 raw[DEPTH];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) raw[i] = *reinterpret_cast<const uint4 *>(at + i * step);
-      at += 4 * step;
+      for (int i = 0; i < DEPTH; ++i) raw[i] = *reinterpret_cast<const uint4 *>(at + i * step);
+      at += DEPTH * step;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) take(raw[i]);
+      for (int i = 0; i < DEPTH; ++i) take(raw[i]);
     }
     for (; k < mine; ++k, at += step) take(*reinterpret_cast<const uint4 *>(at));
   }

@@ -1963,7 +1963,9 @@ public:
     a_.eps = s.eps; a_.act = s.act;
     const int columns = plan_.vecs * (plan_.aligned ? 1 : 16 / (int)in->elsize());
     a_.lanes = plan_.lanes;
-    a_.col_split = std::max(1, (int)plan_.threads / columns);
+    a_.col_split = plan_.col_split;
+    a_.group_span = plan_.group_span;
+    a_.inv_group_width = 1.0f / (plan_.aligned ? a_.cg / (16 / (int)in->elsize()) : a_.cg);
     a_.inv_vecs = 1.0f / plan_.vecs; a_.inv_lanes = 1.0f / plan_.lanes; a_.inv_cg = 1.0f / a_.cg; a_.inv_width = 1.0f / columns;
     a_.vecs = plan_.vecs; a_.chunk_groups = plan_.chunk_groups; a_.chunks = plan_.chunks; a_.parts = plan_.parts; a_.part_pixels = plan_.part_pixels;
     if (plan_.form == NORM_STREAMED) {

@@ -106,6 +106,7 @@ struct GroupNormPlan {
   int nv = 1;             // vectors per thread
   bool aligned = false;   // a vector's channels belong to one group
   int vecs = 1, lanes = 1, chunk_groups = 0, chunks = 0, parts = 1, part_pixels = 0;
+  int col_split = 1, group_span = 32;
   int apply_parts = 1, apply_pixels = 0;
   unsigned apply_grid = 0;
   size_t smem = 0;
@@ -130,7 +131,7 @@ inline GroupNormPlan group_norm_plan(int n, int pixels, int c, int groups, int e
     if (nvec <= 8 * 512) {
       p.form = NORM_ROWS_BLOCK;
       p.threads = 128;
-      while (p.threads < 512 && (int)p.threads * 4 < nvec) p.threads *= 2;
+      while (p.threads < 512 && (int)p.threads * 2 < nvec) p.threads *= 2;
       p.nv = (nvec + p.threads - 1) / p.threads;
       return p;
     }
@@ -154,7 +155,11 @@ inline GroupNormPlan group_norm_plan(int n, int pixels, int c, int groups, int e
     p.nv = (p.part_pixels + p.lanes - 1) / p.lanes;
     p.threads = (unsigned)threads;
     p.grid = (unsigned)((long long)n * p.parts); // x chunks
-    p.smem = ((size_t)threads * per + std::max(threads, p.vecs * per) + round_up(p.chunk_groups, 2)) * 4;
+    // a column's pixel lanes are summed by several threads where there are few columns, eight lanes or more each
+    const int group_width = p.aligned ? cg / N : cg;
+    p.col_split = std::max(1, std::min(threads / (p.vecs * per), p.lanes / 8));
+    p.group_span = round_up(p.col_split * group_width, 32);
+    p.smem = ((size_t)threads * per + (size_t)p.chunk_groups * p.group_span / 32 * 33 + round_up(p.chunk_groups, 2)) * 4;
   };
   // slab: 64 bytes of a pixel and more, at most 8 vectors per thread in at most eight blocks
   const int wide = (4 + unit_vecs - 1) / unit_vecs;
