@@ -57,7 +57,7 @@ __device__ __forceinline__ Pair pair_of_bf16(uint32_t w) { return Pair(__uint_as
 // range.
 __device__ __forceinline__ Pair reciprocals(Pair a) {
   const float r = rcp_approx(a.lo() * a.hi());
-  return Pair(a.hi(), a.lo()) * both(r);
+  return Pair(a.hi() * r, a.lo() * r);
 }
 // v / (1 + 2^t). The exponent is held at 60, so that the product of two denominators stays in range: what is cut off is below
 // 2^-60 of v.
@@ -101,7 +101,7 @@ template <int ACT, bool F32> __device__ __forceinline__ Pair activate(Pair v) {
   return v;
 }
 // `use` is called with the activation as a compile-time constant
-template <class Use> inline void with_activation(int act, Use use) {
+template <class Use> __host__ __device__ inline void with_activation(int act, Use use) {
   switch (act) {
   case ACT_RELU: use(std::integral_constant<int, ACT_RELU>()); break;
   case ACT_SILU: use(std::integral_constant<int, ACT_SILU>()); break;

@@ -72,16 +72,9 @@ template <> struct NormVec<uint16_t> {
   static __device__ __forceinline__ uint16_t back(float v) { return (uint16_t)bf16x2_ieee(v, v); }
 };
 
-// the activation of a vector's values; which one is the same for the whole launch
-template <bool F32, int P> __device__ __forceinline__ void activate_all(int act, Pair (&v)[P]) {
-  auto each = [&](auto k) {
+template <int ACT, bool F32, int P> __device__ __forceinline__ void activate_all(Pair (&v)[P]) {
 #pragma unroll
-    for (int j = 0; j < P; ++j) v[j] = activate<decltype(k)::value, F32>(v[j]);
-  };
-  if (act == ACT_RELU) each(std::integral_constant<int, ACT_RELU>());
-  else if (act == ACT_SILU) each(std::integral_constant<int, ACT_SILU>());
-  else if (act == ACT_GELU) each(std::integral_constant<int, ACT_GELU>());
-  else if (act == ACT_GELU_TANH) each(std::integral_constant<int, ACT_GELU_TANH>());
+  for (int j = 0; j < P; ++j) v[j] = activate<ACT, F32>(v[j]);
 }
 template <int P> __device__ __forceinline__ void load_floats(const float *p, Pair (&v)[P]) {
 #pragma unroll
@@ -90,6 +83,12 @@ template <int P> __device__ __forceinline__ void load_floats(const float *p, Pai
     v[2 * i] = Pair(f.x, f.y);
     v[2 * i + 1] = Pair(f.z, f.w);
   }
+}
+// 16 bytes that this SM reads once: they take no place in its L1 (statistics pass of 1 x 256 x 512 x 512 30.5 -> 23.6 us)
+__device__ __forceinline__ uint4 load_once(const void *p) {
+  uint4 r;
+  asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p) : "memory");
+  return r;
 }
 // zero behind the first `valid` values
 template <int P> __device__ __forceinline__ void clip(Pair (&v)[P], int valid) {
@@ -111,66 +110,141 @@ __device__ __forceinline__ float block_sum(float v, float *red) {
   return warp_sum(v);
 }
 
-// ---- rows: groups of one pixel. BLOCK: a block per group, else a warp. NV: vectors per thread. TAIL: the last vector of a group (there is
-// one group then) ends in padded channels.
-template <typename T, int NV, bool BLOCK, bool TAIL> __global__ void __launch_bounds__(BLOCK ? 512 : 128) group_norm_rows_kernel(const GroupNormArgs a) {
+// ---- rows: groups of one pixel. LANES: 8 or 32 lanes of a warp per R groups, 0: a block. NV: vectors per thread. FULL: every thread has that
+// many, of channels only; the threads' means and squares are then joined in one exchange instead of two.
+// gamma and beta are four times the bytes of a BF16 vector: with one row at a time the L1's data path was 61% busy (4099 x 4096: 15.0 us).
+template <typename T, int NV, int R, int LANES, bool FULL> __global__ void __launch_bounds__(LANES ? 128 : 512) group_norm_rows_kernel(const GroupNormArgs a) {
   typedef NormVec<T> V;
-  __shared__ float red[32];
-  const int lane = BLOCK ? threadIdx.x : threadIdx.x & 31, lanes = BLOCK ? blockDim.x : 32;
-  const int row = BLOCK ? blockIdx.x : blockIdx.x * 4 + (threadIdx.x >> 5);
+  constexpr bool BLOCK = LANES == 0;
+  __shared__ float2 red[R][16];
+  const int lane = BLOCK ? threadIdx.x : threadIdx.x & (LANES - 1), lanes = BLOCK ? blockDim.x : LANES;
+  const int unit = BLOCK ? blockIdx.x : blockIdx.x * (128 / (BLOCK ? 1 : LANES)) + threadIdx.x / (BLOCK ? 1 : LANES); // R images, one of their groups
   pdl_prologue();
-  if (!BLOCK && row >= a.n * a.groups) return;
-  const int img = row / a.groups, g = row - img * a.groups, nvec = (a.cg + V::N - 1) / V::N;
-  const size_t base = (size_t)img * a.cp + (size_t)g * a.cg;
-  const uint4 *in = reinterpret_cast<const uint4 *>((const T *)a.in + base);
-  uint4 *out = reinterpret_cast<uint4 *>((T *)a.out + base);
-  uint4 raw[NV];
+  const int nvec = (a.cg + V::N - 1) / V::N;
+  // (without FULL the first half of the vectors is there all the same: plan)
+  auto has = [&](int k) { return FULL || k < NV / 2 || lane + k * lanes < nvec; };
+  const bool tail = !FULL && a.cg % V::N; // the last vector ends in padded channels, which count as zero
+  auto cut = [&](Pair (&x)[V::P], int k) {
+    if (k >= NV / 2 && tail && lane + k * lanes == nvec - 1) clip(x, a.cg - (lane + k * lanes) * V::N);
+  };
+  const int images = a.groups == 1 ? unit : unit / a.groups, g = unit - images * a.groups, img0 = images * R;
+  auto offset = [&](int r) { return (size_t)(img0 + r) * a.cp + (size_t)g * a.cg + (size_t)lane * V::N; };
+  uint4 raw[R][NV];
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int i = lane + k * lanes;
-    raw[k] = i < nvec ? in[i] : make_uint4(0u, 0u, 0u, 0u);
+  for (int r = 0; r < R; ++r) {
+    const uint4 *in = reinterpret_cast<const uint4 *>((const T *)a.in + offset(r));
+#pragma unroll
+    for (int k = 0; k < NV; ++k) raw[r][k] = has(k) && img0 + r < a.n ? load_once(in + k * lanes) : make_uint4(0u, 0u, 0u, 0u);
   }
-  Pair s2 = both(0.0f);
+  float mean[R], m2[R];
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    Pair x[V::P];
-    V::get(raw[k], x);
-    if (TAIL && (lane + k * lanes + 1) * V::N > a.cg) clip(x, a.cg - (lane + k * lanes) * V::N);
+  for (int r = 0; r < R; ++r) {
+    Pair s = both(0.0f);
 #pragma unroll
-    for (int j = 0; j < V::P; ++j) s2 = s2 + x[j];
+    for (int k = 0; k < NV; ++k) {
+      Pair x[V::P];
+      V::get(raw[r][k], x);
+      cut(x, k);
+#pragma unroll
+      for (int j = 0; j < V::P; ++j) s = s + x[j];
+    }
+    mean[r] = (s.lo() + s.hi()) * (FULL ? 1.0f / (NV * V::N) : a.inv_cg);
   }
-  float s = s2.lo() + s2.hi();
-  s = BLOCK ? block_sum(s, red) : warp_sum(s);
-  const float mean = s / (float)a.cg;
-  s2 = both(0.0f);
+  const int warps = blockDim.x >> 5;
+  // sums over the block (or the warp) of one number per row
+  auto join = [&](float (&v)[R]) {
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    if (lane + k * lanes >= nvec) continue;
-    Pair x[V::P];
-    V::get(raw[k], x);
+    for (int o = 1; o < (BLOCK ? 32 : LANES); o *= 2)
 #pragma unroll
-    for (int j = 0; j < V::P; ++j) x[j] = x[j] + both(-mean);
-    if (TAIL && (lane + k * lanes + 1) * V::N > a.cg) clip(x, a.cg - (lane + k * lanes) * V::N);
+      for (int r = 0; r < R; ++r) v[r] += __shfl_xor_sync(0xffffffffu, v[r], o);
+    if (BLOCK) {
+      __syncthreads();
+      if ((threadIdx.x & 31) == 0)
 #pragma unroll
-    for (int j = 0; j < V::P; ++j) s2 = fma(x[j], x[j], s2);
+        for (int r = 0; r < R; ++r) red[r][threadIdx.x >> 5].x = v[r];
+      __syncthreads();
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        v[r] = 0.0f;
+        for (int w = 0; w < warps; ++w) v[r] += red[r][w].x;
+      }
+    }
+  };
+  if (!FULL) join(mean);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    Pair s = both(0.0f);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if (!has(k)) continue;
+      Pair x[V::P];
+      V::get(raw[r][k], x);
+#pragma unroll
+      for (int j = 0; j < V::P; ++j) x[j] = x[j] + both(-mean[r]);
+      cut(x, k);
+#pragma unroll
+      for (int j = 0; j < V::P; ++j) s = fma(x[j], x[j], s);
+    }
+    m2[r] = s.lo() + s.hi();
   }
-  s = s2.lo() + s2.hi();
-  s = BLOCK ? block_sum(s, red) : warp_sum(s);
-  const float rstd = rsqrtf(s / (float)a.cg + a.eps);
+  if (FULL) {
+    // equal counts: the mean of two is half their sum, and their M2 grows by half the count times the square of the distance
+    float half = 0.5f * NV * V::N;
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int i = lane + k * lanes;
-    if (i >= nvec) continue;
-    Pair x[V::P], ga[V::P], be[V::P];
-    load_floats(a.gamma + g * a.cg + i * V::N, ga);
-    load_floats(a.beta + g * a.cg + i * V::N, be);
-    V::get(raw[k], x);
+    for (int o = 1; o < (BLOCK ? 32 : LANES); o *= 2) {
 #pragma unroll
-    for (int j = 0; j < V::P; ++j) x[j] = fma(fma(x[j], both(rstd), both(-mean * rstd)), ga[j], be[j]);
-    activate_all<V::kF32>(a.act, x);
-    if (TAIL && (i + 1) * V::N > a.cg) clip(x, a.cg - i * V::N);
-    out[i] = V::put(x);
+      for (int r = 0; r < R; ++r) {
+        const float other = __shfl_xor_sync(0xffffffffu, mean[r], o), d = mean[r] - other;
+        m2[r] += __shfl_xor_sync(0xffffffffu, m2[r], o);
+        m2[r] = fmaf(d * half, d, m2[r]);
+        mean[r] = 0.5f * (mean[r] + other);
+      }
+      half *= 2.0f;
+    }
+    if (BLOCK) {
+      if ((threadIdx.x & 31) == 0)
+#pragma unroll
+        for (int r = 0; r < R; ++r) red[r][threadIdx.x >> 5] = make_float2(mean[r], m2[r]);
+      __syncthreads();
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        mean[r] = m2[r] = 0.0f;
+        for (int w = 0; w < warps; ++w) mean[r] += red[r][w].x;
+        mean[r] *= 1.0f / (float)warps;
+        for (int w = 0; w < warps; ++w) {
+          const float2 o = red[r][w];
+          m2[r] += fmaf((o.x - mean[r]) * (32.0f * NV * V::N), o.x - mean[r], o.y);
+        }
+      }
+    }
+  } else {
+    join(m2);
   }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    m2[r] = rsqrtf(fmaf(m2[r], a.inv_cg, a.eps));
+    mean[r] *= -m2[r];
+  }
+  const float *gamma = a.gamma + g * a.cg + lane * V::N, *beta = a.beta + g * a.cg + lane * V::N;
+  with_activation(a.act, [&](auto act) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if (!has(k)) continue;
+      Pair ga[V::P], be[V::P];
+      load_floats(gamma + k * lanes * V::N, ga);
+      load_floats(beta + k * lanes * V::N, be);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        Pair x[V::P];
+        V::get(raw[r][k], x);
+#pragma unroll
+        for (int j = 0; j < V::P; ++j) x[j] = fma(fma(x[j], both(m2[r]), both(mean[r])), ga[j], be[j]);
+        activate_all<decltype(act)::value, V::kF32>(x);
+        cut(x, k);
+        if (img0 + r < a.n) reinterpret_cast<uint4 *>((T *)a.out + offset(r))[k * lanes] = V::put(x);
+      }
+    }
+  });
 }
 
 // ---- what slab and streamed share: a block takes pixels x a chunk; a thread keeps to one vector column
@@ -290,12 +364,12 @@ template <typename T> struct NormAffine {
       }
     }
   }
-  __device__ __forceinline__ uint4 apply(const GroupNormArgs &a, const uint4 &raw, int valid) const {
+  template <int ACT> __device__ __forceinline__ uint4 apply(const uint4 &raw, int valid) const {
     Pair x[V::P];
     V::get(raw, x);
 #pragma unroll
     for (int j = 0; j < V::P; ++j) x[j] = fma(x[j], scale[j], shift[j]);
-    activate_all<V::kF32>(a.act, x);
+    activate_all<ACT, V::kF32>(x);
     if (valid < V::N) clip(x, valid);
     return V::put(x);
   }
@@ -318,7 +392,7 @@ template <typename T, bool ALIGNED, int NV> __global__ void __launch_bounds__(kS
   norm_clear<T, ALIGNED, kSlabThreads>(a, tab);
 #pragma unroll
   for (int k = 0; k < NV; ++k)
-    if (k * t.lanes < mine) raw[k] = *reinterpret_cast<const uint4 *>(in + at + k * step);
+    if (k * t.lanes < mine) raw[k] = load_once(in + at + k * step);
   Pair sum[P];
 #pragma unroll
   for (int j = 0; j < P; ++j) sum[j] = both(0.0f);
@@ -380,16 +454,42 @@ template <typename T, bool ALIGNED, int NV> __global__ void __launch_bounds__(kS
   if (t.active) {
     affine.template set<ALIGNED>(a, t.ch, [&](int g) { return all[g - t.first_group]; });
     T *out = (T *)a.out;
+    with_activation(a.act, [&](auto act) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
-      if (k * t.lanes < mine) *reinterpret_cast<uint4 *>(out + at + k * step) = affine.apply(a, raw[k], ALIGNED ? V::N : a.c - t.ch);
+      for (int k = 0; k < NV; ++k)
+        if (k * t.lanes < mine)
+          *reinterpret_cast<uint4 *>(out + at + k * step) = affine.template apply<decltype(act)::value>(raw[k], ALIGNED ? V::N : a.c - t.ch);
+    });
   }
   __syncwarp();
   if (a.parts > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); // none leaves while its numbers may be read
 }
 
 // ---- streamed
-template <typename T, bool ALIGNED> __global__ void __launch_bounds__(kStreamThreads, 2) group_norm_stats_kernel(const GroupNormArgs a) {
+// use(vector, index) for `count` vectors that are `step` values apart, the next D of them on their way while D are used (with one set of
+// four and no way ahead: 4 x 128 x 128 x 128 12.3 us with three modules in flight instead of 10.7, fp32 2 x 100 x 400 x 400 165 instead of 70).
+template <int D, typename T, class Use> __device__ __forceinline__ void for_vectors(const T *p, long long step, int count, Use use) {
+  uint4 r[2][D];
+  auto fetch = [&](uint4 (&to)[D], int k) {
+#pragma unroll
+    for (int i = 0; i < D; ++i)
+      if (k + i < count) to[i] = load_once(p + (k + i) * step);
+  };
+  auto each = [&](const uint4 (&from)[D], int k) {
+#pragma unroll
+    for (int i = 0; i < D; ++i)
+      if (k + i < count) use(from[i], k + i);
+  };
+  fetch(r[0], 0);
+  for (int k = 0; k < count; k += 2 * D) {
+    fetch(r[1], k + D);
+    each(r[0], k);
+    fetch(r[0], k + 2 * D);
+    each(r[1], k + D);
+  }
+}
+
+template <typename T, bool ALIGNED> __global__ void __launch_bounds__(kStreamThreads, 3) group_norm_stats_kernel(const GroupNormArgs a) {
   extern __shared__ float smem[];
   typedef NormVec<T> V;
   constexpr int P = ALIGNED ? 1 : V::P;
@@ -422,17 +522,7 @@ template <typename T, bool ALIGNED> __global__ void __launch_bounds__(kStreamThr
 #pragma unroll
       for (int j = 0; j < P; ++j) first[j] = ALIGNED ? both(-x[0].lo()) : x[j] * both(-1.0f);
     }
-    int k = 0;
-    constexpr int DEPTH = ALIGNED ? 8 : 4; // loads in flight, as the registers allow
-    for (; k + DEPTH <= mine; k += DEPTH) {
-      uint4 raw[DEPTH];
-#pragma unroll
-      for (int i = 0; i < DEPTH; ++i) raw[i] = *reinterpret_cast<const uint4 *>(at + i * step);
-      at += DEPTH * step;
-#pragma unroll
-      for (int i = 0; i < DEPTH; ++i) take(raw[i]);
-    }
-    for (; k < mine; ++k, at += step) take(*reinterpret_cast<const uint4 *>(at));
+    for_vectors<ALIGNED ? 4 : 2>(at, (long long)step, mine, [&](const uint4 &raw, int) { take(raw); });
   }
   // The thread's count, mean and M2 (per channel; where vectors lie within groups both halves count as columns of their own)
   const float n = (float)mine * (ALIGNED ? V::P : 1), inv = mine > 0 ? 1.0f / n : 0.0f;
@@ -459,7 +549,7 @@ template <typename T, bool ALIGNED> __global__ void __launch_bounds__(kStreamThr
   norm_group_sums<T, ALIGNED, kStreamThreads>(a, t, x, tab, [&](int g, float sum) { partial[(size_t)g * a.parts + t.part] = make_float2(mean_of[g], sum); });
 }
 
-template <typename T, bool ALIGNED> __global__ void __launch_bounds__(kStreamThreads, 2) group_norm_apply_kernel(const GroupNormArgs a) {
+template <typename T, bool ALIGNED> __global__ void __launch_bounds__(kStreamThreads, 3) group_norm_apply_kernel(const GroupNormArgs a) {
   extern __shared__ float smem[];
   float2 *stats = reinterpret_cast<float2 *>(smem); // [groups of the chunk]: mean, 1 / sqrt(var + eps)
   const NormTile<T, kStreamThreads> t(a, gridDim.x - 1 - blockIdx.x, a.apply_parts, a.apply_pixels);
@@ -490,19 +580,13 @@ template <typename T, bool ALIGNED> __global__ void __launch_bounds__(kStreamThr
   const int mine = t.px0 + t.p < t.px1 ? small_div(t.px1 - t.px0 - t.p + t.lanes - 1, a.inv_lanes) : 0, valid = ALIGNED ? NormVec<T>::N : a.c - t.ch;
   const size_t step = (size_t)t.lanes * a.cp;
   // from the last pixel to the first
-  size_t at = t.offset(a, t.px0 + t.p) + (size_t)max(mine - 1, 0) * step;
-  const T *in = (const T *)a.in;
-  T *out = (T *)a.out;
-  int k = 0;
-  for (; k + 4 <= mine; k += 4) {
-    uint4 raw[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) raw[i] = *reinterpret_cast<const uint4 *>(in + at - i * step);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4 *>(out + at - i * step) = affine.apply(a, raw[i], valid);
-    at -= 4 * step;
-  }
-  for (; k < mine; ++k, at -= step) *reinterpret_cast<uint4 *>(out + at) = affine.apply(a, *reinterpret_cast<const uint4 *>(in + at), valid);
+  const size_t at = t.offset(a, t.px0 + t.p) + (size_t)max(mine - 1, 0) * step;
+  T *out = (T *)a.out + at;
+  with_activation(a.act, [&](auto act) {
+    for_vectors<4>((const T *)a.in + at, -(long long)step, mine, [&](const uint4 &raw, int k) {
+      *reinterpret_cast<uint4 *>(out - k * step) = affine.template apply<decltype(act)::value>(raw, valid);
+    });
+  });
 }
 
 // ---- strided: one block per image and group, three passes over its values
@@ -531,20 +615,24 @@ template <typename T> __global__ void group_norm_strided_kernel(const GroupNormA
   for (size_t i = threadIdx.x; i < count; i += blockDim.x) {
     const size_t o = at(i);
     const int ch = g * a.cg + (int)(o % a.cp);
-    Pair v[1] = {both(fmaf((V::one(in[o]) - mean) * rstd, a.gamma[ch], a.beta[ch]))};
-    activate_all<V::kF32>(a.act, v);
-    out[o] = V::back(v[0].lo());
+    const Pair v = both(fmaf((V::one(in[o]) - mean) * rstd, a.gamma[ch], a.beta[ch]));
+    with_activation(a.act, [&](auto act) { out[o] = V::back(activate<decltype(act)::value, V::kF32>(v).lo()); });
   }
 }
 
 inline void launch_group_norm(const GroupNormArgs &a, const GroupNormPlan &p, bool f32, cudaStream_t s) {
   auto by_type = [&](auto type) {
     typedef decltype(type) T;
-    auto rows = [&](auto nv, auto block) {
-      constexpr int NV = decltype(nv)::value;
-      constexpr bool BLOCK = decltype(block)::value;
-      if (a.cg % NormVec<T>::N) launch_k(group_norm_rows_kernel<T, NV, BLOCK, true>, p.grid, p.threads, 0, s, a);
-      else launch_k(group_norm_rows_kernel<T, NV, BLOCK, false>, p.grid, p.threads, 0, s, a);
+    auto rows = [&](auto nv, auto r, auto lanes) {
+      constexpr int NV = decltype(nv)::value, R = decltype(r)::value, LANES = decltype(lanes)::value;
+      if constexpr (NV * R <= 8 && (LANES != 8 || NV <= 2)) {
+        if (a.cg == NV * NormVec<T>::N * (LANES ? LANES : (int)p.threads)) launch_k(group_norm_rows_kernel<T, NV, R, LANES, true>, p.grid, p.threads, 0, s, a);
+        else launch_k(group_norm_rows_kernel<T, NV, R, LANES, false>, p.grid, p.threads, 0, s, a);
+      }
+    };
+    auto by_rows = [&](auto nv, auto lanes) {
+      if (p.rows == 2) rows(nv, std::integral_constant<int, 2>(), lanes);
+      else rows(nv, std::integral_constant<int, 1>(), lanes);
     };
     auto slab = [&](auto nv) {
       constexpr int NV = decltype(nv)::value;
@@ -558,8 +646,11 @@ inline void launch_group_norm(const GroupNormArgs &a, const GroupNormPlan &p, bo
       else use(std::integral_constant<int, 8>());
     };
     switch (p.form) {
-    case NORM_ROWS_WARP: by_nv([&](auto nv) { rows(nv, std::false_type()); }); break;
-    case NORM_ROWS_BLOCK: by_nv([&](auto nv) { rows(nv, std::true_type()); }); break;
+    case NORM_ROWS_WARP:
+      if (p.lanes == 8) by_nv([&](auto nv) { by_rows(nv, std::integral_constant<int, 8>()); });
+      else by_nv([&](auto nv) { by_rows(nv, std::integral_constant<int, 32>()); });
+      break;
+    case NORM_ROWS_BLOCK: by_nv([&](auto nv) { by_rows(nv, std::integral_constant<int, 0>()); }); break;
     case NORM_SLAB: by_nv(slab); break;
     case NORM_STREAMED: {
       auto both_passes = [&](auto aligned) {

@@ -99,11 +99,12 @@ inline LinearSpec linear_spec(const ParsedOp &op, const DevTensor &in, const Dev
 
 // ---- how a group norm runs (group_norm.cuh)
 enum NormForm { NORM_ROWS_WARP = 0, NORM_ROWS_BLOCK, NORM_SLAB, NORM_STREAMED, NORM_STRIDED };
-constexpr int kSlabThreads = 512, kStreamThreads = 512;
+constexpr int kSlabThreads = 512, kStreamThreads = 256;
 struct GroupNormPlan {
   int form = NORM_STRIDED;
   unsigned grid = 0, threads = 256;
   int nv = 1;             // vectors per thread
+  int rows = 1;           // rows forms: rows at a time
   bool aligned = false;   // a vector's channels belong to one group
   int vecs = 1, lanes = 1, chunk_groups = 0, chunks = 0, parts = 1, part_pixels = 0;
   int col_split = 1, group_span = 32;
@@ -119,20 +120,28 @@ inline GroupNormPlan group_norm_plan(int n, int pixels, int c, int groups, int e
   p.aligned = cg % N == 0;
   if (mode == 1 + NORM_STRIDED) return p;
   if (pixels == 1 && (p.aligned || groups == 1) && mode <= 1 + NORM_ROWS_BLOCK) {
-    // a thread keeps up to 8 vectors: a warp 256, a block of up to 512 threads 4096
+    // a thread keeps up to 8 vectors: 8 lanes of a warp, a warp, or a block, which is larger where there are too few rows for all SMs
     const int nvec = (cg + N - 1) / N;
+    const bool many = n >= 8 * sm_count;
+    auto units = [&](int lanes) { // of two neighbouring images where there are many, which share gamma and beta
+      p.nv = 1;
+      while (p.nv * lanes < nvec) p.nv *= 2;
+      p.rows = many && p.nv <= 4 ? 2 : 1;
+      return (long long)((n + p.rows - 1) / p.rows) * groups;
+    };
     if (nvec <= 8 * 32 && mode != 1 + NORM_ROWS_BLOCK) {
       p.form = NORM_ROWS_WARP;
-      p.nv = (nvec + 31) / 32;
       p.threads = 128;
-      p.grid = (unsigned)(((long long)n * groups + 3) / 4);
+      p.lanes = nvec <= 16 ? 8 : 32;
+      const int per_block = 128 / p.lanes;
+      p.grid = (unsigned)((units(p.lanes) + per_block - 1) / per_block);
       return p;
     }
     if (nvec <= 8 * 512) {
       p.form = NORM_ROWS_BLOCK;
-      p.threads = 128;
-      while (p.threads < 512 && (int)p.threads * 2 < nvec) p.threads *= 2;
-      p.nv = (nvec + p.threads - 1) / p.threads;
+      const int want = many ? 4 : 2;
+      p.threads = (unsigned)std::max(64, std::min(512, round_up((nvec + want - 1) / want, 32)));
+      p.grid = (unsigned)units((int)p.threads);
       return p;
     }
   }
@@ -174,13 +183,19 @@ inline GroupNormPlan group_norm_plan(int n, int pixels, int c, int groups, int e
     // ... where its blocks all run at once
     if (mode == 1 + NORM_SLAB || (long long)p.grid * p.chunks <= (p.nv <= 4 ? 2LL : 1LL) * sm_count) return p;
   }
-  // streamed: chunks of whole rows where they fit, and as many parts of the image as fill the SMs; a thread has 8 vectors at least
+  // streamed: chunks of whole rows where they fit, and as many parts of the image as run at once; a thread has 8 vectors at least
   const int most_units = std::max(1, 256 / unit_vecs);
   lay_out(kStreamThreads, most_units, 1);
-  const long long slabs = (long long)n * p.chunks, fill = std::max(1LL, sm_count / slabs), per_part = 8LL * p.lanes;
-  const int parts = (int)std::max(1LL, std::min(fill, (pixels + per_part - 1) / per_part));
-  const int apply = (int)std::max(1LL, std::min(2 * fill, (pixels + per_part - 1) / per_part));
-  lay_out(kStreamThreads, most_units, std::max(parts, (int)((pixels + (1LL << 22) - 1) >> 22))); // (small_div)
+  const long long slabs = (long long)n * p.chunks, per_part = 8LL * p.lanes;
+  auto parts_of = [&](int blocks) { return (int)std::max(1LL, std::min((long long)blocks * sm_count / slabs, (pixels + per_part - 1) / per_part)); };
+  // Blocks per SM of the two passes. Few leave fewer partial statistics and less around the loops, many hide the memory's latency; us alone /
+  // with three modules in flight, (1, 1), (1, 2), (2, 3): 4 x 128 x 128 x 128 24.6 / 10.7, 22.5 / 12.0, 20.5 / 13.8; 8 x 320 x 64 x 64
+  // 28.7 / 14.1, 26.6 / 15.2, 22.6 / 16.5; 1 x 256 x 512 x 512 106 / 65, 91 / 71, 85 / 66; fp32 2 x 100 x 400 x 400 129 / 83, 116 / 83, 90 / 70.
+  // From 128 vectors per thread on the loops are all that counts.
+  const bool large = slabs * pixels * p.vecs >= 128LL * kStreamThreads * sm_count;
+  const int fs = large ? 2 : 1, fa = large ? 3 : 2;
+  const int apply = parts_of(fa);
+  lay_out(kStreamThreads, most_units, std::max(parts_of(fs), (int)((pixels + (1LL << 22) - 1) >> 22))); // (small_div)
   p.apply_pixels = (pixels + std::max(apply, p.parts) - 1) / std::max(apply, p.parts);
   p.apply_parts = (pixels + p.apply_pixels - 1) / p.apply_pixels;
   p.apply_grid = (unsigned)((long long)n * p.apply_parts);
