@@ -278,6 +278,21 @@ def test_linear_tensor_core_forms(M, m, k, n, tiles):
     assert np.array_equal(got, run_linear(M, x, w, bias, "silu", res, options=[("linear_tiles", tiles)]))
 
 
+@pytest.mark.parametrize("rows", [8, 16, 24, 32, 40, 48, 56, 64, 72])
+@pytest.mark.parametrize("split", [1, 2, 3, 8])
+@pytest.mark.parametrize("m,k,n", [(1, 600, 300), (77, 333, 130), (200, 20, 71)])
+def test_linear_fp32_forms(M, m, k, n, split, rows):
+    rng = np.random.default_rng(m + n)
+    x, w = cast(rng.normal(0, 1, (m, k)), "FP32"), cast(rng.normal(0, k ** -0.5, (n, k)), "FP32")
+    bias, res = rng.normal(0, 0.3, n).astype(np.float32), cast(rng.normal(0, 1, (m, n)), "FP32")
+    want, tol = linear_want(x, w, bias, "gelu_tanh", res, "FP32")
+    form, options = {}, [("linear_tiles", 1000 * split + rows)]
+    got = run_linear(M, x, w, bias, "gelu_tanh", res, "FP32", options=options, form=form)
+    assert form == {"tiles": "direct", "rows": min(rows, 64), "channels": 128 if rows == 72 else 64, "split_k": min(split, (k + 15) // 16)}
+    assert_close(got, want, tol)
+    assert np.array_equal(got, run_linear(M, x, w, bias, "gelu_tanh", res, "FP32", options=options))
+
+
 @pytest.mark.parametrize("tiles", [1128, 4064, 10064])
 def test_linear_bounded_wait_runs_out(M, tiles):
     """A hand-over that never comes: the launch ends with a status, the interpreter stays usable."""

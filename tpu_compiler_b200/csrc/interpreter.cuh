@@ -1892,12 +1892,7 @@ public:
     if (names_operand(op, 7)) res_ = I.tensor(op.in[7]);
     const LinearSpec s = linear_spec(op, *in, *out, res_.get(), [&](const std::string &nm) -> const HostWeight & { return I.weight(nm); });
     act_ = s.act;
-    a_ = LinearArgs{};
-    a_.m = s.m; a_.k = s.k_dev; a_.n = s.n; a_.ldy = out->cp;
-    a_.x = in->dev;
-    a_.y = out->dev;
-    a_.res = res_ ? res_->dev : nullptr;
-    a_.bias = I.upload(s.bias);
+    const float *bias = I.upload(s.bias);
     // weights in the device's order of K, (y, x, c) with the input's channel pitch; rows of padded channels are zero
     const size_t k = (size_t)in->c * s.hw;
     auto packed = [&](auto zero, auto conv) {
@@ -1910,7 +1905,12 @@ public:
       }
       return (const void *)I.upload(w);
     };
-    a_.w = out->dtype == DT_F32 ? packed(0.0f, [](float v) { return v; }) : packed((uint16_t)0, [](float v) { return f32_to_bf16_bits(v); });
+    const void *w = out->dtype == DT_F32 ? packed(0.0f, [](float v) { return v; }) : packed((uint16_t)0, [](float v) { return f32_to_bf16_bits(v); });
+    if (out->dtype == DT_F32) {
+      f32_plan_ = linear_f32_plan(s.m, s.k_dev, out->cp, I.sm_count, I.linear_tiles);
+      f32_ = LinearF32Args{(const float *)in->dev, (const float *)w, res_ ? (const float *)res_->dev : nullptr, bias, (float *)out->dev,
+                           s.m, s.k_dev, out->cp, out->cp, f32_plan_.split, s.act};
+    }
     if (out->dtype == DT_BF16) {
       tc_.plan = linear_tc_plan(s.m, s.k_dev, out->cp, I.sm_count, I.linear_tiles);
       const LinearTcPlan &l = tc_.plan;
@@ -1919,14 +1919,14 @@ public:
       p.m = s.m; p.n_pad = p.ldy = out->cp;
       p.k_blocks = l.k_blocks; p.nt = l.nt; p.split = l.split; p.a_rows = l.a_rows; p.stages = l.stages; p.tmem_cols = l.tmem_cols;
       p.idesc = make_idesc_bf16(l.pair ? 256 : 128, l.nt);
-      p.bias = a_.bias;
-      p.res = (const uint16_t *)a_.res;
-      p.y = (uint16_t *)a_.y;
+      p.bias = bias;
+      p.res = res_ ? (const uint16_t *)res_->dev : nullptr;
+      p.y = (uint16_t *)out->dev;
       p.err = &I.ss.d_err->code;
       p.wait_rounds = I.selftest_lost_arrival;
       p.lose_arrival = I.selftest_lost_arrival > 0;
       encode_matrix_map(&tc_.tmX, (const int8_t *)in->dev, s.m, s.k_dev * 2, s.k_dev * 2, 128, l.pair ? 128 : l.a_rows);
-      encode_matrix_map(&tc_.tmW, (const int8_t *)a_.w, out->cp, s.k_dev * 2, s.k_dev * 2, 128, l.pair ? l.nt / 2 : l.nt);
+      encode_matrix_map(&tc_.tmW, (const int8_t *)w, out->cp, s.k_dev * 2, s.k_dev * 2, 128, l.pair ? l.nt / 2 : l.nt);
       linear_kernel_ready(tc_, act_);
     }
     alg_ops = 2.0 * s.m * k * s.n;
@@ -1934,17 +1934,18 @@ public:
   }
   void invoke(cudaStream_t s) override {
     if (out_->dtype == DT_BF16) launch_linear_tc(tc_, act_, s);
-    else launch_linear(a_, true, act_, s);
+    else launch_linear_f32(f32_, f32_plan_, s);
   }
   std::string form() const override {
-    if (out_->dtype != DT_BF16) return "tiles=direct";
+    if (out_->dtype != DT_BF16) return "tiles=direct rows=" + std::to_string(8 * f32_plan_.rm) + " channels=" + std::to_string(16 * f32_plan_.rn) + " split_k=" + std::to_string(f32_plan_.split);
     return std::string("tiles=") + (tc_.plan.pair ? "pair" : "cluster") + " channels=" + std::to_string(tc_.plan.nt) + " split_k=" + std::to_string(tc_.plan.split);
   }
 
 private:
   TensorPtr in_, out_, res_;
-  LinearArgs a_;
   LinearTc tc_;
+  LinearF32Args f32_;
+  LinearF32Plan f32_plan_;
   int act_ = ACT_NONE;
 };
 

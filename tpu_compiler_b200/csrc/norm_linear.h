@@ -245,10 +245,40 @@ inline LinearTcPlan linear_tc_sizes(bool pair, int nt, int split, int m, int k_d
 // mode (option "linear_tiles"): 1 by size; 1000 * split + nt; 10000 + nt: pairs
 inline LinearTcPlan linear_tc_plan(int m, int k_dev, int n_pad, int sm_count, int mode) {
   if (mode >= 10000) return linear_tc_sizes(true, mode - 10000, 1, m, k_dev, n_pad, sm_count);
-  if (mode >= 1000) return linear_tc_sizes(false, mode % 1000, mode / 1000, m, k_dev, n_pad, sm_count);
+  if (mode >= 1000) return linear_tc_sizes(false, round_up(mode % 1000, 16), mode / 1000, m, k_dev, n_pad, sm_count);
   const long long tiles = (long long)((m + 255) / 256) * ((n_pad + 255) / 256);
   if (tiles >= sm_count / 3) return linear_tc_sizes(true, 256, 1, m, k_dev, n_pad, sm_count);
   return linear_tc_sizes(false, 64, 2, m, k_dev, n_pad, sm_count);
+}
+
+// ---- how an fp32 inner product runs (linear.cuh): 8 rm rows x 16 rn channels per tile, `split` blocks share its K
+struct LinearF32Plan {
+  int rm = 8, rn = 4, split = 1;
+  unsigned grid = 0;
+};
+// mode (option "linear_tiles"): 1 by size; 1000 * split + rows of a tile, for fp32 8 to 64, rounded up to a multiple of 8; 72: 64 x 128
+inline LinearF32Plan linear_f32_plan(int m, int k, int n_pad, int sm_count, int mode) {
+  LinearF32Plan best;
+  const int blocks = (k + 15) / 16;
+  double least = 0;
+  for (int form = 1; form <= 9; ++form)
+    for (int split = 1; split <= std::min(8, blocks); ++split) {
+      if (mode >= 1000 && mode < 10000 && (form != std::max(1, std::min(9, (mode % 1000 + 7) / 8)) || split != std::min(std::min(mode / 1000, 8), blocks))) continue;
+      const int rm = std::min(form, 8), rn = form == 9 ? 8 : 4;
+      const long long grid = (long long)((n_pad + 16 * rn - 1) / (16 * rn)) * ((m + 8 * rm - 1) / (8 * rm)) * split;
+      // Clocks of the busiest SM. Per K block of 16 values a block takes 64 (rm + rn) of its shared memory's or, if that is more, 16 rm rn of
+      // the multiply-adds', and 200 at least of its share of the memory's rate; one block alone waits 2000 / stages for its copies.
+      const double on_sm = (double)((grid + sm_count - 1) / sm_count), work = std::max(std::max(64.0 * (rm + rn), 16.0 * rm * rn), 200.0) + 60.0;
+      const double stages = std::min(8, 48 * 1024 / ((8 * rm + 16 * rn) * 80));
+      const double cost = (blocks + split - 1) / split * std::max(on_sm * work, 2000.0 / stages) + on_sm * 300.0 + (split > 1 ? 1500.0 : 0.0);
+      if (least != 0 && cost >= least) continue;
+      least = cost;
+      best.rm = rm;
+      best.rn = rn;
+      best.split = split;
+      best.grid = (unsigned)grid;
+    }
+  return best;
 }
 
 } // namespace tpucb
