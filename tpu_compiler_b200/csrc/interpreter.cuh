@@ -1927,6 +1927,7 @@ public:
       p.lose_arrival = I.selftest_lost_arrival > 0;
       encode_matrix_map(&tc_.tmX, (const int8_t *)in->dev, s.m, s.k_dev * 2, s.k_dev * 2, 128, l.pair ? 128 : l.a_rows);
       encode_matrix_map(&tc_.tmW, (const int8_t *)w, out->cp, s.k_dev * 2, s.k_dev * 2, 128, l.pair ? l.nt / 2 : l.nt);
+      encode_matrix_map(&tc_.tmY, (const int8_t *)out->dev, s.m, out->cp * 2, out->cp * 2, 64, 32);
       linear_kernel_ready(tc_, act_);
     }
     alg_ops = 2.0 * s.m * k * s.n;
@@ -1937,7 +1938,7 @@ public:
     else launch_linear_f32(f32_, f32_plan_, s);
   }
   std::string form() const override {
-    if (out_->dtype != DT_BF16) return "tiles=direct rows=" + std::to_string(8 * f32_plan_.rm) + " channels=" + std::to_string(16 * f32_plan_.rn) + " split_k=" + std::to_string(f32_plan_.split);
+    if (out_->dtype != DT_BF16) return "tiles=direct rows=" + std::to_string(8 * f32_plan_.rm) + " split_k=" + std::to_string(f32_plan_.split);
     return std::string("tiles=") + (tc_.plan.pair ? "pair" : "cluster") + " channels=" + std::to_string(tc_.plan.nt) + " split_k=" + std::to_string(tc_.plan.split);
   }
 

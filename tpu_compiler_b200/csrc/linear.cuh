@@ -2,12 +2,11 @@
 // (Three TF32 products on the tensor cores, as the convolutions have them, lose a factor of 2 to 4 of fp32's precision at these K; calibration,
 // whose pass this is, can wait for the exact one.) Bound: 128 multiply-adds per clock and SM.
 //
-// A block of 128 threads computes 8 RM rows x 16 RN channels, a thread RM x RN of them, 8 rows and 16 channels apart. Both operands lie along
-// K in memory and so in shared memory (rows of 16 values and 4 of padding: eight rows' 16 bytes meet no bank twice); packed multiply-adds
-// take two K at once, so that a sum is two partial ones, of the even and the odd K. Per four K a warp's multiply-adds take 4 RM RN clocks
-// of its quarter of the SM, and its RM + RN reads of 16 bytes per lane 4 clocks each of the whole SM: 8 x 8 balances the two, smaller ones are
-// bound by the reads. A cluster of up to eight blocks shares a tile's K and adds up the partial sums through shared memory in the order
-// of K. RM is the one whose tiles fit the rows best: 200 rows are five tiles of 40, not four of 64.
+// A block of 128 threads computes 8 RM rows x 64 channels, a thread RM x 4 of them, 8 rows and 16 channels apart. Both operands lie along K
+// in memory and so in shared memory (rows of 16 values and 4 of padding: eight rows' 16 bytes meet no bank twice); packed multiply-adds take
+// two K at once, so that a sum is two partial ones, of the even and the odd K. (8 x 8 per thread halve the reads of shared memory, but leave
+// two blocks per SM: 209 us instead of 193 at 2000 x 1000 x 2000; 64 rows spill registers.) A cluster of up to eight blocks shares a tile's K and adds up the partial
+// sums through shared memory in the order of K. RM is the one whose tiles fit the rows best: 200 rows are five tiles of 40, not four of 64.
 #pragma once
 #include "activation.cuh"
 #include "conv_big.cuh"
@@ -22,14 +21,14 @@ struct LinearF32Args {
   int split, act;
 };
 
-constexpr int kF32K = 16, kF32Pitch = kF32K + 4, kF32Threads = 128;
+constexpr int kF32K = 16, kF32Pitch = kF32K + 4, kF32N = 64, kF32Threads = 128;
 // as many stages as 48 KiB hold, eight at most
-__host__ __device__ constexpr int linear_f32_stages(int rm, int rn) {
-  const int fit = 48 * 1024 / ((8 * rm + 16 * rn) * kF32Pitch * 4);
+__host__ __device__ constexpr int linear_f32_stages(int rm) {
+  const int fit = 48 * 1024 / ((8 * rm + kF32N) * kF32Pitch * 4);
   return fit > 8 ? 8 : fit;
 }
-__host__ __device__ constexpr size_t linear_f32_smem(int rm, int rn) {
-  const size_t ring = (size_t)linear_f32_stages(rm, rn) * (8 * rm + 16 * rn) * kF32Pitch * 4, sums = (size_t)8 * rm * 16 * rn * 4;
+__host__ __device__ constexpr size_t linear_f32_smem(int rm) {
+  const size_t ring = (size_t)linear_f32_stages(rm) * (8 * rm + kF32N) * kF32Pitch * 4, sums = (size_t)8 * rm * kF32N * 4;
   return ring > sums ? ring : sums;
 }
 
@@ -40,9 +39,9 @@ __device__ __forceinline__ void cp_async16(uint32_t to, const void *from, bool t
 }
 } // namespace ptx
 
-template <int RM, int RN> __global__ void __launch_bounds__(kF32Threads) linear_f32_kernel(const LinearF32Args a) {
+template <int RM> __global__ void __launch_bounds__(kF32Threads, 4) linear_f32_kernel(const LinearF32Args a) {
   extern __shared__ float smem_f32[];
-  constexpr int BM = 8 * RM, kF32N = 16 * RN, kF32Stages = linear_f32_stages(RM, RN);
+  constexpr int BM = 8 * RM, RN = kF32N / 16, kF32Stages = linear_f32_stages(RM);
   const int rank = (int)ptx::cluster_rank();
   const int n_tiles = (a.n_pad + kF32N - 1) / kF32N, tile = (int)blockIdx.x / a.split, tm = tile / n_tiles;
   const int m0 = tm * BM, n0 = (tile - tm * n_tiles) * kF32N;
@@ -53,22 +52,34 @@ template <int RM, int RN> __global__ void __launch_bounds__(kF32Threads) linear_
   const uint32_t base = ptx::smem_u32(smem_f32);
   constexpr uint32_t kStage = (BM + kF32N) * kF32Pitch * 4, kW = BM * kF32Pitch * 4;
 
-  // rows of four 16-byte pieces
-  auto copy = [&](const float *src, int rows, int row0, int limit, uint32_t to, int kb) {
-    for (int i = threadIdx.x; i < rows * 4; i += kF32Threads) {
-      const int r = i >> 2, c = kb * kF32K + (i & 3) * 4;
-      const bool there = row0 + r < limit && c < a.k;
-      ptx::cp_async16(to + (uint32_t)(r * kF32Pitch + (i & 3) * 4) * 4, there ? src + (size_t)(row0 + r) * a.k + c : src, there);
-    }
+  // Rows of four 16-byte pieces: a thread copies the same piece of every 32nd row, of x and of w. Rows behind the last are those of row 0 (their
+  // results are not written); K behind the last is zero.
+  constexpr int kXCopies = (BM + 31) / 32, kWCopies = kF32N / 32;
+  const int piece = threadIdx.x & 3, row = threadIdx.x >> 2, k_left = a.k - kb0 * kF32K - piece * 4;
+  const float *from_x[kXCopies], *from_w[kWCopies];
+#pragma unroll
+  for (int i = 0; i < kXCopies; ++i) from_x[i] = a.x + (size_t)(m0 + row + 32 * i < a.m ? m0 + row + 32 * i : 0) * a.k + kb0 * kF32K + piece * 4;
+#pragma unroll
+  for (int i = 0; i < kWCopies; ++i) from_w[i] = a.w + (size_t)(n0 + row + 32 * i < a.n_pad ? n0 + row + 32 * i : 0) * a.k + kb0 * kF32K + piece * 4;
+  const uint32_t to = base + (uint32_t)(row * kF32Pitch + piece * 4) * 4;
+  auto copy_w = [&](int it, uint32_t stage) {
+    const bool there = it * kF32K < k_left;
+#pragma unroll
+    for (int i = 0; i < kWCopies; ++i) ptx::cp_async16(to + stage + kW + (uint32_t)(32 * i * kF32Pitch * 4), there ? from_w[i] + it * kF32K : a.w, there);
   };
-  auto copy_w = [&](int i) { copy(a.w, kF32N, n0, a.n_pad, base + (uint32_t)(i % kF32Stages) * kStage + kW, kb0 + i); };
-  auto copy_x = [&](int i) { copy(a.x, BM, m0, a.m, base + (uint32_t)(i % kF32Stages) * kStage, kb0 + i); };
+  auto copy_x = [&](int it, uint32_t stage) {
+    const bool there = it * kF32K < k_left;
+#pragma unroll
+    for (int i = 0; i < kXCopies; ++i)
+      if (BM % 32 == 0 || row + 32 * i < BM)
+        ptx::cp_async16(to + stage + (uint32_t)(32 * i * kF32Pitch * 4), there ? from_x[i] + it * kF32K : a.x, there);
+  };
   for (int i = 0; i < kF32Stages - 1; ++i)
-    if (i < nk) copy_w(i); // weights are written at load time only: they need not wait for the previous kernel
+    if (i < nk) copy_w(i, (uint32_t)i * kStage); // weights are written at load time only: they need not wait for the previous kernel
   pdl_wait();
   pdl_trigger();
   for (int i = 0; i < kF32Stages - 1; ++i) {
-    if (i < nk) copy_x(i);
+    if (i < nk) copy_x(i, (uint32_t)i * kStage);
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
   Pair acc[RM][RN];
@@ -76,15 +87,16 @@ template <int RM, int RN> __global__ void __launch_bounds__(kF32Threads) linear_
   for (int i = 0; i < RM; ++i)
 #pragma unroll
     for (int j = 0; j < RN; ++j) acc[i][j] = both(0.0f);
+  uint32_t stage = 0, next = (kF32Stages - 1) * kStage;
   for (int it = 0; it < nk; ++it) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kF32Stages - 2) : "memory");
     __syncthreads(); // the block's copies of this stage are there, and the stage that comes next has been read by all
     if (it + kF32Stages - 1 < nk) {
-      copy_w(it + kF32Stages - 1);
-      copy_x(it + kF32Stages - 1);
+      copy_w(it + kF32Stages - 1, next);
+      copy_x(it + kF32Stages - 1, next);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
-    const float *xs = smem_f32 + (it % kF32Stages) * (kStage / 4) + ty * kF32Pitch, *ws = smem_f32 + (it % kF32Stages) * (kStage / 4) + kW / 4 + tx * kF32Pitch;
+    const float *xs = smem_f32 + stage / 4 + ty * kF32Pitch, *ws = smem_f32 + (stage + kW) / 4 + tx * kF32Pitch;
 #pragma unroll
     for (int k = 0; k < kF32K; k += 4) {
       float4 x[RM], w[RN];
@@ -95,11 +107,14 @@ template <int RM, int RN> __global__ void __launch_bounds__(kF32Threads) linear_
 #pragma unroll
       for (int i = 0; i < RM; ++i)
 #pragma unroll
-        for (int j = 0; j < RN; ++j) {
-          acc[i][j] = fma(Pair(x[i].x, x[i].y), Pair(w[j].x, w[j].y), acc[i][j]);
-          acc[i][j] = fma(Pair(x[i].z, x[i].w), Pair(w[j].z, w[j].w), acc[i][j]);
-        }
+        for (int j = 0; j < RN; ++j) acc[i][j] = fma(Pair(x[i].x, x[i].y), Pair(w[j].x, w[j].y), acc[i][j]);
+#pragma unroll
+      for (int i = 0; i < RM; ++i)
+#pragma unroll
+        for (int j = 0; j < RN; ++j) acc[i][j] = fma(Pair(x[i].z, x[i].w), Pair(w[j].z, w[j].w), acc[i][j]);
     }
+    stage = stage == (kF32Stages - 1) * kStage ? 0 : stage + kStage;
+    next = next == (kF32Stages - 1) * kStage ? 0 : next + kStage;
   }
   __syncthreads();
 #pragma unroll
@@ -141,22 +156,19 @@ template <int RM, int RN> __global__ void __launch_bounds__(kF32Threads) linear_
 
 inline void launch_linear_f32(const LinearF32Args &a, const LinearF32Plan &p, cudaStream_t s) {
   PdlConvScope conv_class;
-  auto go = [&](auto rm, auto rn) {
-    constexpr int RM = decltype(rm)::value, RN = decltype(rn)::value;
-    static_assert(linear_f32_smem(RM, RN) <= 48 * 1024, "shared memory that a kernel has unasked");
-    launch_cluster_k(p.split, linear_f32_kernel<RM, RN>, p.grid, kF32Threads, linear_f32_smem(RM, RN), s, a);
+  auto go = [&](auto rm) {
+    constexpr int RM = decltype(rm)::value;
+    static_assert(linear_f32_smem(RM) <= 48 * 1024, "shared memory that a kernel has unasked");
+    launch_cluster_k(p.split, linear_f32_kernel<RM>, p.grid, kF32Threads, linear_f32_smem(RM), s, a);
   };
-  std::integral_constant<int, 4> four;
-  switch (p.rm + 8 * (p.rn == 8)) {
-  case 1: go(std::integral_constant<int, 1>(), four); break;
-  case 2: go(std::integral_constant<int, 2>(), four); break;
-  case 3: go(std::integral_constant<int, 3>(), four); break;
-  case 4: go(std::integral_constant<int, 4>(), four); break;
-  case 5: go(std::integral_constant<int, 5>(), four); break;
-  case 6: go(std::integral_constant<int, 6>(), four); break;
-  case 7: go(std::integral_constant<int, 7>(), four); break;
-  case 8: go(std::integral_constant<int, 8>(), four); break;
-  default: go(std::integral_constant<int, 8>(), std::integral_constant<int, 8>());
+  switch (p.rm) {
+  case 1: go(std::integral_constant<int, 1>()); break;
+  case 2: go(std::integral_constant<int, 2>()); break;
+  case 3: go(std::integral_constant<int, 3>()); break;
+  case 4: go(std::integral_constant<int, 4>()); break;
+  case 5: go(std::integral_constant<int, 5>()); break;
+  case 6: go(std::integral_constant<int, 6>()); break;
+  default: go(std::integral_constant<int, 7>());
   }
 }
 

@@ -1,12 +1,14 @@
 // Inner product with bias, activation and residual on the tensor cores: y[m][n] = act(x[m][k] w[n][k]^T + bias) + residual, BF16
 // operands, fp32 accumulators in tensor memory, one rounding.
 //
-// Rows of x lie on the lanes of tensor memory, rows of w (channels) on its columns: an epilogue thread owns a row and writes its
-// channels sixteen at a time, whole 32-byte sectors, with the residual read the same way; nothing passes through shared memory.
+// Rows of x lie on the lanes of tensor memory, rows of w (channels) on its columns: an epilogue thread owns a row, whose residual it reads in
+// whole 32-byte sectors.
 //
 // linear_pair_kernel, for launches of many tiles: a persistent pair of CTAs (two SMs, tcgen05 cta_group::2) computes tiles of 256
 //   rows x nt channels; each CTA holds 128 of the rows and half of the channels' weights, so that a K block of 64 costs an SM
-//   (128 + nt / 2) x 128 bytes of copies. Accumulators are double-buffered: the epilogue of a tile runs beside the next one's loop.
+//   (128 + nt / 2) x 128 bytes of copies. Accumulators are double-buffered: the epilogue of a tile runs beside the next one's loop; its
+//   warps write 32 rows x 32 channels through shared memory by bulk tensor stores, clipped by their map (sectors stored by the threads:
+//   8192 x 256 x 8192 59 us, XX).
 // linear_split_kernel, for the others, down to one row: tiles of 128 rows x nt channels, and a cluster of up to eight CTAs that
 //   share a tile's K, so that few rows still draw weights through all SMs. The partial sums meet in shared memory: every CTA adds up
 //   its share of the columns from all of the cluster, in the order of K (no atomics, the same bits every time), and finishes it.
@@ -25,12 +27,12 @@ struct LinearTcParams {
   int m, n_pad;   // rows; channels with the padding of the pitch, whose weights and bias are zero
   int ldy;        // pitch of y and the residual, in values
   int k_blocks;   // of 64 values
-  int nt;         // channels per tile: a multiple of 16 (pair: of 32), at most 256
+  int nt;         // channels per tile: a multiple of 16 (pair: of 64), at most 256
   int split;      // CTAs that share a tile's K
   int a_rows;     // rows of x per copy
   int stages;
   uint32_t tmem_cols, idesc;
-  const float *bias;
+  const float *bias;   // for whole tiles of 256 channels
   const uint16_t *res; // or null
   uint16_t *y;
   int *err;
@@ -50,6 +52,17 @@ __device__ __forceinline__ void st_global_32b(void *p, const uint32_t (&r)[8]) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
                "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
 }
+__device__ __forceinline__ void tcgen05_ld_x32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, "
+      "%29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
@@ -57,23 +70,28 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
 }
 } // namespace ptx
 
-// Sixteen channels of one row: bias, activation, residual, rounding, one sector.
-template <int ACT> __device__ __forceinline__ void linear_finish16(const float *acc, const LinearTcParams &p, int row, int col) {
-  const size_t at = (size_t)row * p.ldy + col;
-  uint32_t r[8], o[8];
-  if (p.res) ptx::ld_global_32b(p.res + at, r);
+// Sixteen channels of one row: bias, activation, residual, rounding.
+template <int ACT> __device__ __forceinline__ void linear_finish16(const uint32_t *acc, const LinearTcParams &p, size_t at, int col, uint32_t (&o)[8]) {
+  uint32_t r[8];
+  const bool residual = p.res && col < p.n_pad;
+  if (residual) ptx::ld_global_32b(p.res + at, r);
   const float4 *bias = reinterpret_cast<const float4 *>(p.bias + col);
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const float4 b = __ldg(bias + q);
-    Pair v[2] = {activate<ACT, false>(Pair(acc[4 * q], acc[4 * q + 1]) + Pair(b.x, b.y)),
-                 activate<ACT, false>(Pair(acc[4 * q + 2], acc[4 * q + 3]) + Pair(b.z, b.w))};
+    Pair v[2] = {activate<ACT, false>(Pair(__uint_as_float(acc[4 * q]), __uint_as_float(acc[4 * q + 1])) + Pair(b.x, b.y)),
+                 activate<ACT, false>(Pair(__uint_as_float(acc[4 * q + 2]), __uint_as_float(acc[4 * q + 3])) + Pair(b.z, b.w))};
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      if (p.res) v[j] = v[j] + pair_of_bf16(r[2 * q + j]);
+      if (residual) v[j] = v[j] + pair_of_bf16(r[2 * q + j]);
       o[2 * q + j] = bf16x2_ieee(v[j].lo(), v[j].hi());
     }
   }
+}
+template <int ACT> __device__ __forceinline__ void linear_store16(const uint32_t *acc, const LinearTcParams &p, int row, int col) {
+  const size_t at = (size_t)row * p.ldy + col;
+  uint32_t o[8];
+  linear_finish16<ACT>(acc, p, at, col, o);
   ptx::st_global_32b(p.y + at, o);
 }
 
@@ -213,7 +231,7 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
         ptx::tcgen05_ld_x16(acc + (uint32_t)c, r);
         ptx::tcgen05_wait_ld();
         if (p.split == 1) {
-          if (m0 + row < p.m) linear_finish16<ACT>(reinterpret_cast<const float *>(r), p, m0 + row, n0 + c);
+          if (m0 + row < p.m) linear_store16<ACT>(r, p, m0 + row, n0 + c);
           __syncwarp();
         } else {
 #pragma unroll
@@ -244,7 +262,7 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
 #pragma unroll
           for (int j = 0; j < 16; ++j) acc[j] += ptx::ld_cluster_f32(from + 4u * (uint32_t)(j * rows));
         }
-        linear_finish16<ACT>(acc, p, m0 + row, n0 + c);
+        linear_store16<ACT>(reinterpret_cast<const uint32_t *>(acc), p, m0 + row, n0 + c);
       }
     }
     __syncwarp();
@@ -254,14 +272,15 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
 
 template <int ACT>
 __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
-linear_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const LinearTcParams p) {
+linear_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmY,
+                   const LinearTcParams p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = ptx::smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   uint8_t *smem = smem_raw + (base - raw);
   const uint32_t bar_full = base, bar_empty = base + 128, bar_acc_full = base + 256, bar_acc_empty = base + 272;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + 288);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + 292);
-  const uint32_t ring = base + kLinearHeader;
+  const uint32_t ring = base + kLinearHeader + kPairStaging;
 
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = ptx::cluster_rank();
@@ -366,9 +385,9 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
     }
   } else if (warp >= 4) {
     const int quarter = warp & 3, half = (warp - 4) >> 2, row = quarter * 32 + lane;
-    const uint32_t lead_acc_empty = ptx::map_cluster(bar_acc_empty, 0);
+    const uint32_t lead_acc_empty = ptx::map_cluster(bar_acc_empty, 0), out = base + kLinearHeader + (uint32_t)(warp - 4) * 4096u;
     pdl_wait(); // the residual
-    int t = 0;
+    int t = 0, flip = 0;
     for (int tile = first; tile < total; tile += step, ++t) {
       const int tm = tile / n_tiles, tn = tile - tm * n_tiles, buf = t & 1;
       const int m0 = tm * 256 + (int)rank * 128, n0 = tn * p.nt;
@@ -381,14 +400,43 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
       }
       ptx::tcgen05_fence_after();
       if (m0 + quarter * 32 < p.m) {
+        // half of the tile's columns, 32 at a time: the next ones are read while these are finished, and two buffers take turns
         const uint32_t acc = tmem + (uint32_t)buf * 256u + ((uint32_t)(quarter * 32) << 16);
-        const int cols = min(p.nt, p.n_pad - n0);
-        for (int c = half * 16; c < cols; c += 32) {
-          uint32_t r[16];
-          ptx::tcgen05_ld_x16(acc + (uint32_t)c, r);
+        const int c0 = half * (p.nt / 2), steps = min(p.nt / 64, (p.n_pad - n0 - c0 + 31) / 32); // (may be negative)
+        const bool mine = m0 + row < p.m;
+        uint32_t r[2][32];
+        if (steps > 0) ptx::tcgen05_ld_x32(acc + (uint32_t)c0, r[0]);
+        auto finish = [&](const uint32_t (&now)[32], uint32_t (&then)[32], int i) {
+          const int c = c0 + i * 32;
           ptx::tcgen05_wait_ld();
-          if (m0 + row < p.m) linear_finish16<ACT>(reinterpret_cast<const float *>(r), p, m0 + row, n0 + c);
+          if (i + 1 < steps) ptx::tcgen05_ld_x32(acc + (uint32_t)c + 32u, then);
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); // the store before the last has read this buffer
           __syncwarp();
+          const uint32_t to = out + (uint32_t)flip * 2048u + (uint32_t)lane * 64u;
+          flip ^= 1;
+          if (mine) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              uint32_t o[8];
+              // (columns behind the last are clipped by the map; there is bias for them, and no residual)
+              linear_finish16<ACT>(now + 16 * q, p, (size_t)(m0 + row) * p.ldy + n0 + c + 16 * q, n0 + c + 16 * q, o);
+              // the map's 64-byte swizzle: a row's piece i of 16 bytes lies at i ^ (row / 2 % 4)
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + (uint32_t)(((2 * q + j) ^ ((lane >> 1) & 3)) << 4)), "r"(o[4 * j]),
+                             "r"(o[4 * j + 1]), "r"(o[4 * j + 2]), "r"(o[4 * j + 3]) : "memory");
+            }
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            ptx::tma_store_2d(&tmY, to, 2 * (n0 + c), m0 + quarter * 32);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+        };
+        for (int i = 0; i < steps; i += 2) {
+          finish(r[0], r[1], i);
+          if (i + 1 < steps) finish(r[1], r[0], i + 1);
         }
       }
       ptx::tcgen05_fence_before();
@@ -396,6 +444,8 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
       if (lane == 0 && !p.lose_arrival)
         asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(lead_acc_empty + 8 * buf) : "memory");
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
   }
 
   ptx::tcgen05_fence_before();
@@ -408,7 +458,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
 }
 
 struct LinearTc {
-  CUtensorMap tmX, tmW;
+  CUtensorMap tmX, tmW, tmY;
   LinearTcParams p;
   LinearTcPlan plan;
 };
@@ -431,8 +481,11 @@ inline void linear_kernel_ready(const LinearTc &l, int act) {
 inline void launch_linear_tc(const LinearTc &l, int act, cudaStream_t stream) {
   PdlConvScope conv_class;
   with_linear_kernel(l, act, [&](auto k) {
-    launch_cluster_k(l.plan.pair ? 1 : l.plan.split, decltype(k)::value, l.plan.grid, l.plan.pair ? kPairThreads : kSplitThreads, l.plan.smem, stream, l.tmX,
-                     l.tmW, l.p);
+    constexpr auto kernel = decltype(k)::value;
+    if constexpr (std::is_invocable_v<decltype(kernel), CUtensorMap, CUtensorMap, CUtensorMap, LinearTcParams>)
+      launch_k(kernel, l.plan.grid, kPairThreads, l.plan.smem, stream, l.tmX, l.tmW, l.tmY, l.p);
+    else
+      launch_cluster_k(l.plan.split, kernel, l.plan.grid, kSplitThreads, l.plan.smem, stream, l.tmX, l.tmW, l.p);
   });
 }
 

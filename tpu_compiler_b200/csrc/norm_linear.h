@@ -61,7 +61,7 @@ struct LinearSpec {
   int m = 0, n = 0, act = ACT_NONE;
   int hw = 1;         // pixels of an input row: K is hw x channels
   int k_dev = 0;      // K on the device, with the input's channel pitch
-  std::vector<float> bias; // with the result's channel pitch
+  std::vector<float> bias; // zero behind the channels, for whole tiles of 256
   const HostWeight *filter = nullptr;
 };
 inline LinearSpec linear_spec(const ParsedOp &op, const DevTensor &in, const DevTensor &out, const DevTensor *res, const WeightOf &weight) {
@@ -85,7 +85,7 @@ inline LinearSpec linear_spec(const ParsedOp &op, const DevTensor &in, const Dev
   s.k_dev = s.hw * in.cp;
   const size_t k = (size_t)in.c * s.hw;
   TPUCB_CHECK(s.filter->data.size() == s.n * k, "fc %s: filter has %zu values, expected n*k = %zu", nm, s.filter->data.size(), s.n * k);
-  s.bias.assign(out.cp, 0.0f);
+  s.bias.assign(round_up(out.cp, 256), 0.0f);
   if (names_operand(op, 2)) {
     const auto &b = weight(op.in[2]).data;
     TPUCB_CHECK(b.size() == (size_t)s.n, "fc %s: bias has %zu values, expected %d", nm, b.size(), s.n);
@@ -205,7 +205,8 @@ inline GroupNormPlan group_norm_plan(int n, int pixels, int c, int groups, int e
 
 // ---- how an inner product runs on the tensor cores (linear_tc.cuh)
 constexpr int kLinearMaxStages = 16;
-constexpr int kLinearHeader = 1024; // barriers
+constexpr int kLinearHeader = 1024;      // barriers
+constexpr int kPairStaging = 8 * 4096;   // results on their way out, twice 32 rows x 32 channels per epilogue warp
 struct LinearTcPlan {
   bool pair = false;  // two SMs per tile of 256 rows, persistent; else one of 128, and `split` CTAs share its K
   int nt = 0, split = 1, a_rows = 128, stages = 0, k_blocks = 0;
@@ -223,8 +224,8 @@ inline LinearTcPlan linear_tc_sizes(bool pair, int nt, int split, int m, int k_d
   if (pair) {
     const size_t stage = (size_t)(128 + nt / 2) * 128;
     const long long tiles = n_tiles * ((m + 255) / 256);
-    l.stages = (int)std::min<size_t>(kLinearMaxStages, (226 * 1024 - kLinearHeader - 1024) / stage);
-    l.smem = 1024 + kLinearHeader + l.stages * stage; // (more than half of an SM's: two pairs on the same SMs would wait for each other's tensor memory)
+    l.stages = (int)std::min<size_t>(kLinearMaxStages, (227 * 1024 - kLinearHeader - kPairStaging - 1024) / stage);
+    l.smem = 1024 + kLinearHeader + kPairStaging + l.stages * stage; // (more than half of an SM's: two pairs on the same SMs would wait for each other's tensor memory)
     l.grid = (unsigned)(2 * std::min<long long>(tiles, sm_count / 2));
     return l;
   }
@@ -251,30 +252,28 @@ inline LinearTcPlan linear_tc_plan(int m, int k_dev, int n_pad, int sm_count, in
   return linear_tc_sizes(false, 64, 2, m, k_dev, n_pad, sm_count);
 }
 
-// ---- how an fp32 inner product runs (linear.cuh): 8 rm rows x 16 rn channels per tile, `split` blocks share its K
+// ---- how an fp32 inner product runs (linear.cuh): 8 rm rows x 64 channels per tile, `split` blocks share its K
 struct LinearF32Plan {
-  int rm = 8, rn = 4, split = 1;
+  int rm = 1, split = 1;
   unsigned grid = 0;
 };
-// mode (option "linear_tiles"): 1 by size; 1000 * split + rows of a tile, for fp32 8 to 64, rounded up to a multiple of 8; 72: 64 x 128
+// mode (option "linear_tiles"): 1 by size; 1000 * split + rows of a tile, for fp32 8 to 56, rounded up to a multiple of 8
 inline LinearF32Plan linear_f32_plan(int m, int k, int n_pad, int sm_count, int mode) {
   LinearF32Plan best;
   const int blocks = (k + 15) / 16;
   double least = 0;
-  for (int form = 1; form <= 9; ++form)
+  for (int rm = 1; rm <= 7; ++rm)
     for (int split = 1; split <= std::min(8, blocks); ++split) {
-      if (mode >= 1000 && mode < 10000 && (form != std::max(1, std::min(9, (mode % 1000 + 7) / 8)) || split != std::min(std::min(mode / 1000, 8), blocks))) continue;
-      const int rm = std::min(form, 8), rn = form == 9 ? 8 : 4;
-      const long long grid = (long long)((n_pad + 16 * rn - 1) / (16 * rn)) * ((m + 8 * rm - 1) / (8 * rm)) * split;
-      // Clocks of the busiest SM. Per K block of 16 values a block takes 64 (rm + rn) of its shared memory's or, if that is more, 16 rm rn of
-      // the multiply-adds', and 200 at least of its share of the memory's rate; one block alone waits 2000 / stages for its copies.
-      const double on_sm = (double)((grid + sm_count - 1) / sm_count), work = std::max(std::max(64.0 * (rm + rn), 16.0 * rm * rn), 200.0) + 60.0;
-      const double stages = std::min(8, 48 * 1024 / ((8 * rm + 16 * rn) * 80));
-      const double cost = (blocks + split - 1) / split * std::max(on_sm * work, 2000.0 / stages) + on_sm * 300.0 + (split > 1 ? 1500.0 : 0.0);
+      if (mode >= 1000 && mode < 10000 && (rm != std::max(1, std::min(7, (mode % 1000 + 7) / 8)) || split != std::min(std::min(mode / 1000, 8), blocks))) continue;
+      const long long grid = (long long)((n_pad + 63) / 64) * ((m + 8 * rm - 1) / (8 * rm)) * split;
+      // Clocks of an SM, halfway between the busiest one's and the average. Per K block of 16 values a block takes about 96 rm of its multiply-adds
+      // and what copies and barriers cost; alone on its SM it waits 2000 / stages for its copies and gets half of the multiply-adds' rate.
+      const double ratio = (double)grid / sm_count, on_sm = 0.5 * (std::ceil(ratio) + std::max(1.0, ratio)), work = std::max(96.0 * rm + 150.0, 200.0);
+      const double stages = std::min(8, 48 * 1024 / ((8 * rm + 64) * 80)), alone = std::max(2000.0 / stages, 2.0 * 96.0 * rm + 150.0);
+      const double cost = (blocks + split - 1) / split * std::max(on_sm * work, alone) + on_sm * 500.0 + (split > 1 ? 1500.0 : 0.0);
       if (least != 0 && cost >= least) continue;
       least = cost;
       best.rm = rm;
-      best.rn = rn;
       best.split = split;
       best.grid = (unsigned)grid;
     }

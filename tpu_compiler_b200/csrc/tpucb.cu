@@ -397,9 +397,9 @@ int tpucb_interp_set_option(tpucb_interp *it, const char *key, int value) {
     it->impl.norm_form = value; // takes effect at the next load_module
   } else if (k == "linear_tiles") {
     const int nt = value >= 10000 ? value - 10000 : value % 1000, split = value / 1000;
-    TPUCB_CHECK(value == 1 || (value >= 10000 ? nt >= 32 && nt <= 256 && nt % 32 == 0 : split >= 1 && split <= 8 && nt >= 8 && nt <= 256 && nt % 8 == 0),
-                "linear_tiles: 1 (by size, the default), 1000 * CTAs per tile (1 .. 8) + channels (16 .. 256, a multiple of 16; fp32: rows, 8 .. 64, of 8, 72 for 64 x 128) or "
-                "10000 + channels (32 .. 256, a multiple of 32: pairs)");
+    TPUCB_CHECK(value == 1 || (value >= 10000 ? nt >= 64 && nt <= 256 && nt % 64 == 0 : split >= 1 && split <= 8 && nt >= 8 && nt <= 256 && nt % 8 == 0),
+                "linear_tiles: 1 (by size, the default), 1000 * CTAs per tile (1 .. 8) + channels (16 .. 256, a multiple of 16; fp32: rows, 8 .. 56, of 8) or "
+                "10000 + channels (64, 128, 192, 256: pairs)");
     it->impl.linear_tiles = value; // takes effect at the next load_module
   } else if (k == "fuse_activations") {
     it->impl.fuse_activations = value != 0; // takes effect at the next load_module
