@@ -40,7 +40,7 @@ struct LinearTcParams {
 };
 
 constexpr int kSplitThreads = 192;  // copies, MMAs, four epilogue warps
-constexpr int kPairEpilogueWarps = 8;
+constexpr int kPairEpilogueWarps = 16;
 constexpr int kPairThreads = 32 * (4 + kPairEpilogueWarps); // copies of x, of w, MMAs, one idle
 
 namespace ptx {
@@ -384,10 +384,10 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
       }
     }
   } else if (warp >= 4) {
-    const int quarter = warp & 3, half = (warp - 4) >> 2, row = quarter * 32 + lane;
-    const uint32_t lead_acc_empty = ptx::map_cluster(bar_acc_empty, 0), out = base + kLinearHeader + (uint32_t)(warp - 4) * 4096u;
+    const int quarter = warp & 3, part = (warp - 4) >> 2, row = quarter * 32 + lane;
+    const uint32_t lead_acc_empty = ptx::map_cluster(bar_acc_empty, 0), out = base + kLinearHeader + (uint32_t)(warp - 4) * 2048u;
     pdl_wait(); // the residual
-    int t = 0, flip = 0;
+    int t = 0;
     for (int tile = first; tile < total; tile += step, ++t) {
       const int tm = tile / n_tiles, tn = tile - tm * n_tiles, buf = t & 1;
       const int m0 = tm * 256 + (int)rank * 128, n0 = tn * p.nt;
@@ -400,43 +400,34 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
       }
       ptx::tcgen05_fence_after();
       if (m0 + quarter * 32 < p.m) {
-        // half of the tile's columns, 32 at a time: the next ones are read while these are finished, and two buffers take turns
         const uint32_t acc = tmem + (uint32_t)buf * 256u + ((uint32_t)(quarter * 32) << 16);
-        const int c0 = half * (p.nt / 2), steps = min(p.nt / 64, (p.n_pad - n0 - c0 + 31) / 32); // (may be negative)
+        const int cols = min(p.nt, p.n_pad - n0);
         const bool mine = m0 + row < p.m;
-        uint32_t r[2][32];
-        if (steps > 0) ptx::tcgen05_ld_x32(acc + (uint32_t)c0, r[0]);
-        auto finish = [&](const uint32_t (&now)[32], uint32_t (&then)[32], int i) {
-          const int c = c0 + i * 32;
+        for (int c = part * 32; c < cols; c += 128) {
+          uint32_t r[32];
+          ptx::tcgen05_ld_x32(acc + (uint32_t)c, r);
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); // the last store has read the buffer
           ptx::tcgen05_wait_ld();
-          if (i + 1 < steps) ptx::tcgen05_ld_x32(acc + (uint32_t)c + 32u, then);
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); // the store before the last has read this buffer
           __syncwarp();
-          const uint32_t to = out + (uint32_t)flip * 2048u + (uint32_t)lane * 64u;
-          flip ^= 1;
           if (mine) {
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
               uint32_t o[8];
               // (columns behind the last are clipped by the map; there is bias for them, and no residual)
-              linear_finish16<ACT>(now + 16 * q, p, (size_t)(m0 + row) * p.ldy + n0 + c + 16 * q, n0 + c + 16 * q, o);
+              linear_finish16<ACT>(r + 16 * q, p, (size_t)(m0 + row) * p.ldy + n0 + c + 16 * q, n0 + c + 16 * q, o);
               // the map's 64-byte swizzle: a row's piece i of 16 bytes lies at i ^ (row / 2 % 4)
 #pragma unroll
               for (int j = 0; j < 2; ++j)
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + (uint32_t)(((2 * q + j) ^ ((lane >> 1) & 3)) << 4)), "r"(o[4 * j]),
-                             "r"(o[4 * j + 1]), "r"(o[4 * j + 2]), "r"(o[4 * j + 3]) : "memory");
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(out + (uint32_t)lane * 64u + (uint32_t)(((2 * q + j) ^ ((lane >> 1) & 3)) << 4)),
+                             "r"(o[4 * j]), "r"(o[4 * j + 1]), "r"(o[4 * j + 2]), "r"(o[4 * j + 3]) : "memory");
             }
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0) {
-            ptx::tma_store_2d(&tmY, to, 2 * (n0 + c), m0 + quarter * 32);
+            ptx::tma_store_2d(&tmY, out, 2 * (n0 + c), m0 + quarter * 32);
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
-        };
-        for (int i = 0; i < steps; i += 2) {
-          finish(r[0], r[1], i);
-          if (i + 1 < steps) finish(r[1], r[0], i + 1);
         }
       }
       ptx::tcgen05_fence_before();

@@ -206,7 +206,7 @@ inline GroupNormPlan group_norm_plan(int n, int pixels, int c, int groups, int e
 // ---- how an inner product runs on the tensor cores (linear_tc.cuh)
 constexpr int kLinearMaxStages = 16;
 constexpr int kLinearHeader = 1024;      // barriers
-constexpr int kPairStaging = 8 * 4096;   // results on their way out, twice 32 rows x 32 channels per epilogue warp
+constexpr int kPairStaging = 16 * 2048;  // results on their way out, 32 rows x 32 channels per epilogue warp
 struct LinearTcPlan {
   bool pair = false;  // two SMs per tile of 256 rows, persistent; else one of 128, and `split` CTAs share its K
   int nt = 0, split = 1, a_rows = 128, stages = 0, k_blocks = 0;
