@@ -1912,8 +1912,7 @@ public:
                            s.m, s.k_dev, out->cp, out->cp, f32_plan_.split, s.act};
     }
     if (out->dtype == DT_BF16) {
-      tc_.plan = linear_tc_plan(s.m, s.k_dev, out->cp, I.sm_count, I.linear_tiles);
-      const LinearTcPlan &l = tc_.plan;
+      const LinearTcPlan &l = tc_.plan = linear_tc_plan(s.m, s.k_dev, out->cp, I.sm_count, I.linear_tiles);
       LinearTcParams &p = tc_.p;
       p = LinearTcParams{};
       p.m = s.m; p.n_pad = p.ldy = out->cp;
@@ -1939,7 +1938,8 @@ public:
   }
   std::string form() const override {
     if (out_->dtype != DT_BF16) return "tiles=direct rows=" + std::to_string(8 * f32_plan_.rm) + " split_k=" + std::to_string(f32_plan_.split);
-    return std::string("tiles=") + (tc_.plan.pair ? "pair" : "cluster") + " channels=" + std::to_string(tc_.plan.nt) + " split_k=" + std::to_string(tc_.plan.split);
+    const LinearTcPlan &l = tc_.plan;
+    return std::string("tiles=") + (l.pair ? "pair" : "cluster") + " channels=" + std::to_string(l.nt) + " split_k=" + std::to_string(l.split);
   }
 
 private:

@@ -244,14 +244,28 @@ inline LinearTcPlan linear_tc_sizes(bool pair, int nt, int split, int m, int k_d
   return l;
 }
 // mode (option "linear_tiles"): 1 by size; 1000 * split + nt; 10000 + nt: pairs
+// By size; us with three modules in flight / alone:
+//   Pairs where there are more tiles of 128 x 64 than SMs, and more than one of rows; 256 channels, 128 where those leave half of the
+//   pairs idle. 256 x 4096 x 16384 31 / 37 (clusters of one 35 / 62), 8192 x 4096 x 4096 190 / 180 (222 / 240), 600 x 1000 x 5000 8.8 / 14.4 (8.8 /
+//   18.3), 2048 x 512 x 2048 7.1 / 10.3 (6.7 / 12.3); 512 x 4096 x 4096 with 256 channels 14.0 / 26.8, with 128 15.6 / 18.6.
+//   Else as many clusters as the SMs hold. Sharing K pays from about twelve K blocks per CTA on; below, and up to 64 CTAs, narrower tiles do:
+//   256 x 1024 x 1024 with 32 channels 2.7 / 8.2, with 64 and two CTAs 4.0 / 10.2; 1 x 4096 x 4096 with 128 channels and four CTAs 6.2 / 12.3, with 64
+//   and two 9.0 / 14.3, with 32 and one 7.0 / 16.4; 1 x 1024 x 1024 3.2 / 8.2. The exchange grows with the rows: 128 x 4096 x 4096 with 128 and
+//   four 8.6 / 16.3, with 64 and two 8.1 / 14.3.
 inline LinearTcPlan linear_tc_plan(int m, int k_dev, int n_pad, int sm_count, int mode) {
   if (mode >= 10000) return linear_tc_sizes(true, mode - 10000, 1, m, k_dev, n_pad, sm_count);
   if (mode >= 1000) return linear_tc_sizes(false, round_up(mode % 1000, 16), mode / 1000, m, k_dev, n_pad, sm_count);
-  const long long tiles = (long long)((m + 255) / 256) * ((n_pad + 255) / 256);
-  if (tiles >= sm_count / 3) return linear_tc_sizes(true, 256, 1, m, k_dev, n_pad, sm_count);
-  return linear_tc_sizes(false, 64, 2, m, k_dev, n_pad, sm_count);
+  auto tiles = [&](int rows, int nt) { return (long long)((m + rows - 1) / rows) * ((n_pad + nt - 1) / nt); };
+  if (m > 128 && tiles(128, 64) > sm_count) return linear_tc_sizes(true, tiles(256, 256) > sm_count / 4 ? 256 : 128, 1, m, k_dev, n_pad, sm_count);
+  const int most = std::max(1, (k_dev + 63) / 64 / 12);
+  int nt = m <= 32 ? 128 : 64, split;
+  for (;; nt /= 2) {
+    nt = std::min(nt, round_up(n_pad, 16));
+    split = (int)std::max(1LL, std::min<long long>(std::min(8, most), sm_count / tiles(128, nt)));
+    if (nt <= 16 || tiles(128, nt) * split >= 64) break;
+  }
+  return linear_tc_sizes(false, round_up(nt, 16), split, m, k_dev, n_pad, sm_count);
 }
-
 // ---- how an fp32 inner product runs (linear.cuh): 8 rm rows x 64 channels per tile, `split` blocks share its K
 struct LinearF32Plan {
   int rm = 1, split = 1;
