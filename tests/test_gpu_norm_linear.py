@@ -141,6 +141,22 @@ def test_group_norm_forms(M, form, shape, groups, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["BF16", "FP32"])
+@pytest.mark.parametrize("form,shape,groups", [
+    ("slab", (1, 320, 96, 100), 32), ("slab", (1, 96, 70, 111), 8), ("slab", (2, 64, 90, 90), 2), ("slab", (150, 64, 20, 20), 32),  # most of shared memory
+    ("streamed", (1, 512, 40, 60), 512), ("streamed", (1, 2048, 20, 21), 2048), ("streamed", (1, 2100, 20, 21), 300),  # many groups per row
+    ("strided", (1, 524400, 2, 1), 8)])  # more channels than the others divide
+def test_group_norm_at_its_limits(M, form, shape, groups, dtype):
+    rng = np.random.default_rng(31)
+    x = cast(rng.normal(0, 1, shape) + rng.normal(0, 1, (1, shape[1], 1, 1)), dtype)
+    gamma, beta = rng.normal(1, 0.3, shape[1]).astype(np.float32), rng.normal(0, 0.3, shape[1]).astype(np.float32)
+    want, tol = norm_want(x, groups, gamma, beta, 1e-5, "gelu", dtype)
+    took = {}
+    options = [("norm_form", 0 if form == "strided" else 1 + NORM_FORMS.index(form))]
+    assert_close(run_norm(M, x, groups, gamma, beta, act="gelu", dtype=dtype, options=options, form=took), want, tol)
+    assert took["form"] == form
+
+
+@pytest.mark.parametrize("dtype", ["BF16", "FP32"])
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("shape,groups", [((6, 256), 1), ((2, 64, 6, 6), 4)])
 def test_group_norm_activations_far_out(M, shape, groups, act, dtype):

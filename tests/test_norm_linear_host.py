@@ -156,3 +156,94 @@ def test_oracle_definitions_against_torch(act):
     w, bias, r = rng.normal(0, 1, (7, 15)), rng.normal(0, 1, 7), rng.normal(0, 1, (24, 7))
     want = (f(torch.tensor(rows) @ torch.tensor(w).T + torch.tensor(bias)) + torch.tensor(r)).numpy()
     assert np.abs(O.linear64(rows, w, bias, act, r) - want).max() < 2 ** -45 * 64
+
+
+PLANS = r"""
+#include "norm_linear.h"
+#include <iostream>
+using namespace tpucb;
+#define EXPECT(x) do { if (!(x)) { std::cout << #x << " fails for " << what << std::endl; return 1; } } while (0)
+int norm(int n, int pixels, int c, int groups, int es, int sms, int mode) {
+  std::stringstream ss;
+  ss << "n " << n << " pixels " << pixels << " c " << c << " groups " << groups << " es " << es << " sms " << sms << " mode " << mode;
+  const std::string what = ss.str();
+  const GroupNormPlan p = group_norm_plan(n, pixels, c, groups, es, sms, mode);
+  const int N = 16 / es, cg = c / groups, nvec = (cg + N - 1) / N;
+  if (p.form == NORM_ROWS_WARP || p.form == NORM_ROWS_BLOCK) {
+    const bool warp = p.form == NORM_ROWS_WARP;
+    const int lanes = warp ? p.lanes : (int)p.threads;
+    EXPECT(pixels == 1 && (cg % N == 0 || groups == 1));
+    EXPECT(p.nv <= 8 && p.nv * lanes >= nvec && (p.nv == 1 || p.nv / 2 * lanes < nvec));
+    EXPECT((long long)p.grid * (warp ? p.threads / p.lanes : 1) >= (long long)((n + p.rows - 1) / p.rows) * groups);
+    EXPECT(p.threads % 32 == 0 && p.threads <= 512 && (p.rows == 1 || p.nv <= 4));
+  } else if (p.form == NORM_SLAB || p.form == NORM_STREAMED) {
+    const bool slab = p.form == NORM_SLAB;
+    EXPECT(p.threads == (slab ? kSlabThreads : kStreamThreads));
+    EXPECT(p.chunks <= 65535 && p.chunk_groups >= 1 && p.chunk_groups <= 256 && (long long)p.chunks * p.chunk_groups >= groups);
+    EXPECT((p.chunks - 1) * p.chunk_groups < groups);
+    EXPECT((long long)p.vecs * N >= (long long)p.chunk_groups * cg && (p.chunks == 1 || p.chunk_groups * cg == p.vecs * N));
+    EXPECT(p.lanes >= 1 && p.vecs * p.lanes <= (int)p.threads && p.nv * p.lanes >= p.part_pixels && p.col_split >= 1);
+    EXPECT((long long)p.parts * p.part_pixels >= pixels && (long long)(p.parts - 1) * p.part_pixels < pixels);
+    EXPECT(p.grid == (unsigned)(n * p.parts) && p.part_pixels <= 1 << 22);
+    const int per = p.aligned ? 1 : N, group_width = p.aligned ? cg / N : cg;
+    EXPECT(p.group_span % 32 == 0 && p.group_span >= p.col_split * group_width);
+    const size_t tab = ((size_t)p.threads * per + (size_t)p.chunk_groups * (p.group_span + p.group_span / 32)) * 4;
+    if (slab) {
+      EXPECT(p.parts <= 8 && p.smem <= 227 * 1024);
+      EXPECT(p.smem >= tab + (size_t)p.nv * kSlabThreads * 16 + (size_t)p.chunk_groups * 16);
+    } else {
+      EXPECT(p.smem <= 48 * 1024 && p.smem >= tab + (size_t)p.chunk_groups * 4 && p.smem >= (size_t)p.chunk_groups * 8);
+      EXPECT((long long)p.apply_parts * p.apply_pixels >= pixels && (long long)(p.apply_parts - 1) * p.apply_pixels < pixels);
+      EXPECT(p.apply_grid == (unsigned)(n * p.apply_parts) && p.apply_pixels <= 1 << 22);
+    }
+  } else EXPECT(p.grid == (unsigned)(n * groups));
+  return 0;
+}
+int linear(int m, int k, int n, int sms, int mode) {
+  std::stringstream ss;
+  ss << "m " << m << " k " << k << " n " << n << " sms " << sms << " mode " << mode;
+  const std::string what = ss.str();
+  const int n_pad = round_up(n, 16);
+  const LinearTcPlan l = linear_tc_plan(m, k, n_pad, sms, mode);
+  EXPECT(l.nt >= 16 && l.nt <= 256 && l.nt % (l.pair ? 64 : 16) == 0 && l.split >= 1 && l.split <= 8);
+  EXPECT(l.split <= (k + 63) / 64 && (l.pair ? l.split == 1 : true));
+  EXPECT(l.smem <= 227 * 1024 && l.stages <= kLinearMaxStages && l.stages >= std::min(2, (l.k_blocks + l.split - 1) / l.split));
+  EXPECT((l.tmem_cols & (l.tmem_cols - 1)) == 0 && l.tmem_cols >= 32 && l.tmem_cols <= 512 && (int)l.tmem_cols >= l.nt * (l.pair ? 2 : 1));
+  EXPECT(l.pair || (l.a_rows >= std::min(m, 128) && l.a_rows <= 128 && l.a_rows % 8 == 0));
+  const LinearF32Plan f = linear_f32_plan(m, k, n, sms, mode);
+  EXPECT(f.rm >= 1 && f.rm <= 7 && f.split >= 1 && f.split <= 8);
+  return 0;
+}
+int main() {
+  const int channels[] = {1, 3, 7, 8, 16, 33, 62, 64, 100, 320, 512, 1025, 2048, 4100, 8192, 20000, 524287, 600000};
+  const int pixels[] = {1, 2, 9, 64, 1767, 4096, 10000, 90000, 262144, 50000000};
+  for (int c : channels)
+    for (int g = 1; g <= c; g = g < 64 ? g + 1 : g * 2)
+      for (int px : pixels)
+        for (int n : {1, 2, 9, 300, 8192})
+          for (int es : {2, 4})
+            for (int mode = 0; mode <= 5; ++mode)
+              for (int sms : {148, 20})
+                if (c % g == 0 && (long long)c * px * n < 1LL << 36 && (long long)n * g < 1LL << 31 && norm(n, px, c, g, es, sms, mode)) return 1;
+  for (int c : {512, 2048, 8192, 524287, 524286})
+    for (int es : {2, 4})
+      for (int mode = 0; mode <= 5; ++mode)
+        if (norm(3, 12000, c, c, es, 148, mode)) return 1;
+  for (int m : {1, 2, 17, 128, 129, 200, 256, 1000, 4100, 100000})
+    for (int k : {1, 16, 64, 700, 768, 1000, 4096, 8192, 100000})
+      for (int n : {1, 16, 17, 60, 250, 1000, 2050, 4096, 16384, 300000})
+        for (int mode : {1, 1016, 2064, 8256, 3048, 5080, 10064, 10128, 10192, 10256})
+          for (int sms : {148, 20})
+            if (linear(m, k, n, sms, mode)) return 1;
+  std::cout << "sound" << std::endl;
+}
+"""
+
+
+def test_plans_cover_their_tensors_within_the_limits(tmp_path):
+    """Every pixel, channel and group has a block, shared and tensor memory suffice, grids stay within what a launch may have."""
+    src, exe = tmp_path / "t.cpp", str(tmp_path / "t")
+    src.write_text(PLANS)
+    subprocess.run(["g++", "-O1", "-std=c++17", "-I", os.path.join(ROOT, "tpu_compiler_b200", "csrc"), "-I", "/usr/local/cuda/include",
+                    str(src), "-o", exe], check=True)
+    assert subprocess.run([exe], capture_output=True, text=True).stdout.strip() == "sound"

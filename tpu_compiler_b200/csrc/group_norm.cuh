@@ -6,8 +6,8 @@
 //
 // Four forms (group_norm_plan), threads moving vectors of 16 bytes:
 //   rows     one pixel per image: a group is contiguous; a warp or a block keeps it in registers;
-//   slab     the pixels of an image x a few groups ("chunk") are kept in the registers of a cluster of up to eight blocks, which
-//            exchange their statistics through shared memory: x is read once;
+//   slab     the pixels of an image x a few groups ("chunk") are kept in the shared memory of a cluster of up to eight blocks, which
+//            exchange their statistics through it: x is read once;
 //   streamed larger ones: a pass for the statistics of parts of an image, and a pass that joins them and forms the results, in the
 //            opposite order, so that it begins with what the L2 still holds;
 //   strided  what fits no whole vectors: a block per group, three passes.
@@ -19,7 +19,7 @@
 // The result is one multiply-add per value, with beta - mean rstd gamma rounded once, an error like that of the mean itself.
 #pragma once
 #include "activation.cuh"
-#include "conv_big.cuh"
+#include "conv_plan.cuh"
 
 namespace tpucb {
 
@@ -31,6 +31,7 @@ struct GroupNormArgs {
   float eps;
   int act;
   // slab and streamed: chunks of `vecs` vectors = whole groups (the last may have fewer), `parts` blocks share an image's pixels
+  int held; // slab: vectors per thread
   int vecs, lanes, chunk_groups, chunks, parts, part_pixels; // (lanes: pixels that a block's threads take at once)
   int apply_parts, apply_pixels; // streamed: of the second pass
   int col_split, group_span;     // norm_group_sums: threads per column; parts of columns per group, rounded up to whole warps
@@ -337,6 +338,58 @@ __device__ __forceinline__ void own_means(const GroupNormArgs &a, int ch, int fi
     for (int j = 0; j < NormVec<T>::P; ++j) m[j] = Pair(v[2 * j], v[2 * j + 1]);
   }
 }
+// What a thread sums: distances from its first value and their squares, per channel or, where vectors lie within groups, in all.
+template <typename T, bool ALIGNED> struct NormMoments {
+  typedef NormVec<T> V;
+  static constexpr int P = ALIGNED ? 1 : V::P;
+  Pair first[P] = {}, s[P] = {}, q[P] = {}; // first: negative
+  __device__ __forceinline__ void begin(const uint4 &raw) {
+    Pair x[V::P];
+    V::get(raw, x);
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      first[j] = ALIGNED ? both(-x[0].lo()) : x[j] * both(-1.0f);
+      s[j] = q[j] = both(0.0f);
+    }
+  }
+  __device__ __forceinline__ void take(const uint4 &raw) {
+    Pair x[V::P];
+    V::get(raw, x);
+#pragma unroll
+    for (int j = 0; j < V::P; ++j) {
+      const int i = ALIGNED ? 0 : j;
+      const Pair d = x[j] + first[i];
+      s[i] = s[i] + d;
+      q[i] = fma(d, d, q[i]);
+    }
+  }
+  // The block's mean and M2 of each group of its chunk, from `mine` vectors of each thread: `done(group of the chunk, mean, M2)` in one thread
+  // each. mean_of: [groups of the chunk]; tab: norm_group_sums. (Where vectors lie within groups both halves of the pairs count as columns.)
+  template <int THREADS, class Done>
+  __device__ __forceinline__ void join(const GroupNormArgs &a, const NormTile<T, THREADS> &t, int mine, float *mean_of, float *tab, Done done) {
+    const float n = (float)mine * (ALIGNED ? V::P : 1), inv = mine > 0 ? 1.0f / n : 0.0f;
+    const float inv_count = 1.0f / ((float)(t.px1 - t.px0) * (float)a.cg);
+    Pair x[P];
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      const Pair mean = s[j] * both(inv);
+      q[j] = fma(s[j] * both(-1.0f), mean, q[j]);
+      q[j] = Pair(q[j].lo() < 0.0f ? 0.0f : q[j].lo(), q[j].hi() < 0.0f ? 0.0f : q[j].hi()); // (a NaN stays)
+      first[j] = fma(first[j], both(-1.0f), mean); // the mean
+      x[j] = mine > 0 ? first[j] * both(n) : both(0.0f);
+    }
+    norm_group_sums<T, ALIGNED, THREADS>(a, t, x, tab, [&](int g, float sum) { mean_of[g] = sum * inv_count; });
+    __syncthreads();
+    Pair m[P];
+    own_means<T, ALIGNED>(a, t.ch, t.first_group, t.n_groups, [&](int g) { return mean_of[g]; }, m);
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      const Pair d = first[j] + m[j];
+      x[j] = mine > 0 ? fma(d * both(n), d, q[j]) : both(0.0f);
+    }
+    norm_group_sums<T, ALIGNED, THREADS>(a, t, x, tab, [&](int g, float sum) { done(g, mean_of[g], sum); });
+  }
+};
 // y = x scale + shift of a thread's channels
 template <typename T> struct NormAffine {
   typedef NormVec<T> V;
@@ -375,90 +428,73 @@ template <typename T> struct NormAffine {
   }
 };
 
-// ---- slab. ALIGNED: a vector's channels belong to one group. NV: vectors per thread.
-template <typename T, bool ALIGNED, int NV> __global__ void __launch_bounds__(kSlabThreads, NV <= 4 ? 2 : 1) group_norm_slab_kernel(const GroupNormArgs a) {
-  typedef NormVec<T> V;
-  extern __shared__ float smem[];
-  float2 *own = reinterpret_cast<float2 *>(smem); // [groups of the chunk]: this block's mean and M2
-  float2 *all = own + a.chunk_groups;             // mean and 1 / sqrt(var + eps) of the image
+// ---- slab. ALIGNED: a vector's channels belong to one group. A thread's vectors wait in shared memory, [vector][thread], where it alone writes
+// and reads them: no barrier orders them. Bound by the memory's latency and the sums between its two halves, which other blocks of the SM fill where
+// there are any: 64 x 256 x 32 x 32 with SiLU 14.2 us with three modules in flight (72% of the memory's rate), 8 x 320 x 64 x 64 12.8, alone
+// 18.5. (With the vectors in registers, eight per thread, those took 22.8, 25.1 and 28.7 us: a wave of blocks held half as much, in one block
+// per SM.)
+template <typename T, bool ALIGNED> __global__ void __launch_bounds__(kSlabThreads, 2) group_norm_slab_kernel(const GroupNormArgs a) {
+  extern __shared__ __align__(16) float smem[];
+  uint4 *held = reinterpret_cast<uint4 *>(smem) + threadIdx.x;
+  float2 *own = reinterpret_cast<float2 *>(smem + (size_t)a.held * kSlabThreads * 4); // [groups of the chunk]: this block's mean and M2
+  float2 *all = own + a.chunk_groups;                                                 // mean and 1 / sqrt(var + eps) of the image
   float *tab = reinterpret_cast<float *>(all + a.chunk_groups);
   const NormTile<T, kSlabThreads> t(a, blockIdx.x, a.parts, a.part_pixels);
-  constexpr int P = ALIGNED ? 1 : V::P;
   const size_t at = t.offset(a, t.px0 + t.p), step = (size_t)t.lanes * a.cp;
-  const int mine = t.active ? t.px1 - t.px0 - t.p : 0; // pixels from the thread's first on
-  pdl_prologue();
-  const T *in = (const T *)a.in;
-  uint4 raw[NV];
+  const int mine = t.active && t.px0 + t.p < t.px1 ? small_div(t.px1 - t.px0 - t.p + t.lanes - 1, a.inv_lanes) : 0;
   norm_clear<T, ALIGNED, kSlabThreads>(a, tab);
-#pragma unroll
-  for (int k = 0; k < NV; ++k)
-    if (k * t.lanes < mine) raw[k] = load_once(in + at + k * step);
-  Pair sum[P];
-#pragma unroll
-  for (int j = 0; j < P; ++j) sum[j] = both(0.0f);
-#pragma unroll
-  for (int k = 0; k < NV; ++k)
-    if (k * t.lanes < mine) {
-      Pair x[V::P];
-      V::get(raw[k], x);
-#pragma unroll
-      for (int j = 0; j < V::P; ++j) sum[ALIGNED ? 0 : j] = sum[ALIGNED ? 0 : j] + x[j];
-    }
-  const float inv_count = 1.0f / ((float)(t.px1 - t.px0) * (float)a.cg);
-  norm_group_sums<T, ALIGNED, kSlabThreads>(a, t, sum, tab, [&](int g, float s) { own[g].x = s * inv_count; });
-  __syncthreads();
-  Pair mean_of[P]; // negative
-  own_means<T, ALIGNED>(a, t.ch, t.first_group, t.n_groups, [&](int g) { return own[g].x; }, mean_of);
-#pragma unroll
-  for (int j = 0; j < P; ++j) sum[j] = both(0.0f);
-#pragma unroll
-  for (int k = 0; k < NV; ++k)
-    if (k * t.lanes < mine) {
-      Pair x[V::P];
-      V::get(raw[k], x);
-#pragma unroll
-      for (int j = 0; j < V::P; ++j) {
-        const Pair d = x[j] + mean_of[ALIGNED ? 0 : j];
-        sum[ALIGNED ? 0 : j] = fma(d, d, sum[ALIGNED ? 0 : j]);
-      }
-    }
-  norm_group_sums<T, ALIGNED, kSlabThreads>(a, t, sum, tab, [&](int g, float s) { own[g].y = s; });
+  pdl_prologue();
+  {
+    const T *in = (const T *)a.in + at;
+    uint32_t to = ptx::smem_u32(held);
+#pragma unroll 4
+    for (int k = 0; k < mine; ++k, in += step, to += kSlabThreads * 16)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(in) : "memory");
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  }
+  NormMoments<T, ALIGNED> moments;
+  moments.begin(mine > 0 ? held[0] : make_uint4(0u, 0u, 0u, 0u));
+#pragma unroll 4
+  for (int k = 0; k < mine; ++k) moments.take(held[k * kSlabThreads]);
+  float *mean_of = reinterpret_cast<float *>(all);
+  moments.template join<kSlabThreads>(a, t, mine, mean_of, tab, [&](int g, float mean, float m2) { own[g] = make_float2(mean, m2); });
   NormAffine<T> affine;
   if (t.active) affine.load(a, t.ch);
   if (a.parts > 1) ptx::cluster_sync();
   else __syncthreads();
   const float total = (float)a.pixels * (float)a.cg;
-  for (int g = threadIdx.x; g < t.n_groups; g += kSlabThreads) {
-    float mean = own[g].x, m2 = own[g].y;
-    if (a.parts > 1) {
-      auto pixels_of = [&](int r) { return (float)(min((r + 1) * a.part_pixels, a.pixels) - r * a.part_pixels); };
-      auto other = [&](int r) {
-        float2 o;
-        const uint32_t at = ptx::map_cluster(ptx::smem_u32(&own[g]), (uint32_t)r);
-        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(o.x), "=f"(o.y) : "r"(at) : "memory");
-        return o;
-      };
-      mean = m2 = 0.0f;
-#pragma unroll 1
-      for (int r = 0; r < a.parts; ++r) mean += other(r).x * (pixels_of(r) / (float)a.pixels);
-#pragma unroll 1
-      for (int r = 0; r < a.parts; ++r) {
-        const float2 o = other(r);
-        m2 += fmaf((o.x - mean) * (o.x - mean), pixels_of(r) * (float)a.cg, o.y);
-      }
+  if (a.parts == 1) {
+    for (int g = threadIdx.x; g < t.n_groups; g += kSlabThreads) all[g] = make_float2(own[g].x, rsqrtf(own[g].y / total + a.eps));
+  } else {
+    // eight threads per group, one block's numbers each (a thread that read them all took a round trip for each: 2 x 320 x 96 x 96 by 8
+    // blocks 12.7 us with three modules in flight instead of 11.3)
+    const int r = threadIdx.x & 7;
+    const float share = r < a.parts ? (float)(min((r + 1) * a.part_pixels, a.pixels) - r * a.part_pixels) : 0.0f;
+    auto sum8 = [](float v) {
+#pragma unroll
+      for (int k = 4; k; k /= 2) v += __shfl_xor_sync(0xffffffffu, v, k);
+      return v;
+    };
+    for (int first = 0; first < t.n_groups; first += kSlabThreads / 8) {
+      const int g = min(first + (int)threadIdx.x / 8, t.n_groups - 1);
+      float2 o = make_float2(0.0f, 0.0f);
+      if (r < a.parts)
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(o.x), "=f"(o.y) : "r"(ptx::map_cluster(ptx::smem_u32(&own[g]), (uint32_t)r)) : "memory");
+      const float mean = sum8(o.x * (share / (float)a.pixels)), d = o.x - mean;
+      const float m2 = sum8(r < a.parts ? fmaf(d * d, share * (float)a.cg, o.y) : 0.0f);
+      if (r == 0) all[g] = make_float2(mean, rsqrtf(m2 / total + a.eps)); // (several threads of the last group write the same)
     }
-    all[g] = make_float2(mean, rsqrtf(m2 / total + a.eps));
   }
   __syncthreads();
   if (a.parts > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); // the others' numbers have been read
   if (t.active) {
     affine.template set<ALIGNED>(a, t.ch, [&](int g) { return all[g - t.first_group]; });
     T *out = (T *)a.out;
+    const int valid = ALIGNED ? NormVec<T>::N : a.c - t.ch;
     with_activation(a.act, [&](auto act) {
-#pragma unroll
-      for (int k = 0; k < NV; ++k)
-        if (k * t.lanes < mine)
-          *reinterpret_cast<uint4 *>(out + at + k * step) = affine.template apply<decltype(act)::value>(raw[k], ALIGNED ? V::N : a.c - t.ch);
+#pragma unroll 2
+      for (int k = 0; k < mine; ++k)
+        *reinterpret_cast<uint4 *>(out + at + k * step) = affine.template apply<decltype(act)::value>(held[k * kSlabThreads], valid);
     });
   }
   __syncwarp();
@@ -466,9 +502,10 @@ template <typename T, bool ALIGNED, int NV> __global__ void __launch_bounds__(kS
 }
 
 // ---- streamed
-// use(vector, index) for `count` vectors that are `step` values apart, the next D of them on their way while D are used (with one set of
+// begin(the first vector) and use(vector, index) for `count` vectors that are `step` values apart, the next D of them on their way while D are used (with one set of
 // four and no way ahead: 4 x 128 x 128 x 128 12.3 us with three modules in flight instead of 10.7, fp32 2 x 100 x 400 x 400 165 instead of 70).
-template <int D, typename T, class Use> __device__ __forceinline__ void for_vectors(const T *p, long long step, int count, Use use) {
+template <int D, typename T, class Begin, class Use>
+__device__ __forceinline__ void for_vectors(const T *p, long long step, int count, Begin begin, Use use) {
   uint4 r[2][D];
   auto fetch = [&](uint4 (&to)[D], int k) {
 #pragma unroll
@@ -481,6 +518,7 @@ template <int D, typename T, class Use> __device__ __forceinline__ void for_vect
       if (k + i < count) use(from[i], k + i);
   };
   fetch(r[0], 0);
+  begin(r[0][0]);
   for (int k = 0; k < count; k += 2 * D) {
     fetch(r[1], k + D);
     each(r[0], k);
@@ -491,62 +529,18 @@ template <int D, typename T, class Use> __device__ __forceinline__ void for_vect
 
 template <typename T, bool ALIGNED> __global__ void __launch_bounds__(kStreamThreads, 3) group_norm_stats_kernel(const GroupNormArgs a) {
   extern __shared__ float smem[];
-  typedef NormVec<T> V;
-  constexpr int P = ALIGNED ? 1 : V::P;
   const NormTile<T, kStreamThreads> t(a, blockIdx.x, a.parts, a.part_pixels);
   float *mean_of = smem; // [groups of the chunk]
   float *tab = smem + (a.chunk_groups + 1) / 2 * 2;
   norm_clear<T, ALIGNED, kStreamThreads>(a, tab);
   pdl_prologue();
   const int mine = t.active && t.px0 + t.p < t.px1 ? small_div(t.px1 - t.px0 - t.p + t.lanes - 1, a.inv_lanes) : 0;
-  Pair first[P], s[P], q[P]; // first: negative
-#pragma unroll
-  for (int j = 0; j < P; ++j) first[j] = s[j] = q[j] = both(0.0f);
-  auto take = [&](const uint4 &raw) {
-    Pair x[V::P];
-    V::get(raw, x);
-#pragma unroll
-    for (int j = 0; j < V::P; ++j) {
-      const int i = ALIGNED ? 0 : j;
-      const Pair d = x[j] + first[i];
-      s[i] = s[i] + d;
-      q[i] = fma(d, d, q[i]);
-    }
-  };
-  if (mine > 0) {
-    const T *at = (const T *)a.in + t.offset(a, t.px0 + t.p);
-    const size_t step = (size_t)t.lanes * a.cp;
-    {
-      Pair x[V::P];
-      V::get(*reinterpret_cast<const uint4 *>(at), x);
-#pragma unroll
-      for (int j = 0; j < P; ++j) first[j] = ALIGNED ? both(-x[0].lo()) : x[j] * both(-1.0f);
-    }
-    for_vectors<ALIGNED ? 4 : 2>(at, (long long)step, mine, [&](const uint4 &raw, int) { take(raw); });
-  }
-  // The thread's count, mean and M2 (per channel; where vectors lie within groups both halves count as columns of their own)
-  const float n = (float)mine * (ALIGNED ? V::P : 1), inv = mine > 0 ? 1.0f / n : 0.0f;
-  const float inv_count = 1.0f / ((float)(t.px1 - t.px0) * (float)a.cg);
-  Pair x[P];
-#pragma unroll
-  for (int j = 0; j < P; ++j) {
-    const Pair mean = s[j] * both(inv);
-    q[j] = fma(s[j] * both(-1.0f), mean, q[j]);
-    q[j] = Pair(q[j].lo() < 0.0f ? 0.0f : q[j].lo(), q[j].hi() < 0.0f ? 0.0f : q[j].hi()); // (a NaN stays)
-    first[j] = fma(first[j], both(-1.0f), mean); // the mean
-    x[j] = first[j] * both(n);
-  }
-  norm_group_sums<T, ALIGNED, kStreamThreads>(a, t, x, tab, [&](int g, float sum) { mean_of[g] = sum * inv_count; });
-  __syncthreads();
-  Pair m[P];
-  own_means<T, ALIGNED>(a, t.ch, t.first_group, t.n_groups, [&](int g) { return mean_of[g]; }, m);
-#pragma unroll
-  for (int j = 0; j < P; ++j) {
-    const Pair d = first[j] + m[j];
-    x[j] = mine > 0 ? fma(d * both(n), d, q[j]) : both(0.0f);
-  }
+  const T *in = (const T *)a.in + (mine > 0 ? t.offset(a, t.px0 + t.p) : 0);
+  NormMoments<T, ALIGNED> moments;
+  if (mine > 0) for_vectors<ALIGNED ? 4 : 2>(in, (long long)t.lanes * a.cp, mine, [&](const uint4 &raw) { moments.begin(raw); }, [&](const uint4 &raw, int) { moments.take(raw); });
   float2 *partial = a.partial + ((size_t)t.img * a.groups + t.first_group) * a.parts;
-  norm_group_sums<T, ALIGNED, kStreamThreads>(a, t, x, tab, [&](int g, float sum) { partial[(size_t)g * a.parts + t.part] = make_float2(mean_of[g], sum); });
+  moments.template join<kStreamThreads>(a, t, mine, mean_of, tab,
+                                        [&](int g, float mean, float m2) { partial[(size_t)g * a.parts + t.part] = make_float2(mean, m2); });
 }
 
 template <typename T, bool ALIGNED> __global__ void __launch_bounds__(kStreamThreads, 3) group_norm_apply_kernel(const GroupNormArgs a) {
@@ -583,7 +577,7 @@ template <typename T, bool ALIGNED> __global__ void __launch_bounds__(kStreamThr
   const size_t at = t.offset(a, t.px0 + t.p) + (size_t)max(mine - 1, 0) * step;
   T *out = (T *)a.out + at;
   with_activation(a.act, [&](auto act) {
-    for_vectors<4>((const T *)a.in + at, -(long long)step, mine, [&](const uint4 &raw, int k) {
+    for_vectors<4>((const T *)a.in + at, -(long long)step, mine, [](const uint4 &) {}, [&](const uint4 &raw, int k) {
       *reinterpret_cast<uint4 *>(out - k * step) = affine.template apply<decltype(act)::value>(raw, valid);
     });
   });
@@ -620,6 +614,20 @@ template <typename T> __global__ void group_norm_strided_kernel(const GroupNormA
   }
 }
 
+// To be called at load, on the device that will run it (conv_kernel_ready).
+inline void group_norm_ready(const GroupNormPlan &p, bool f32) {
+  if (p.form != NORM_SLAB) return;
+  int device = 0;
+  TPUCB_CUDA(cudaGetDevice(&device));
+  auto set = [&](auto k) {
+    static OncePerDevice ready; // one of each kernel
+    ready.run(device, [] { TPUCB_CUDA(cudaFuncSetAttribute(decltype(k)::value, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024)); });
+  };
+  if (f32 && p.aligned) set(KernelConstant<group_norm_slab_kernel<float, true>>());
+  else if (f32) set(KernelConstant<group_norm_slab_kernel<float, false>>());
+  else if (p.aligned) set(KernelConstant<group_norm_slab_kernel<uint16_t, true>>());
+  else set(KernelConstant<group_norm_slab_kernel<uint16_t, false>>());
+}
 inline void launch_group_norm(const GroupNormArgs &a, const GroupNormPlan &p, bool f32, cudaStream_t s) {
   auto by_type = [&](auto type) {
     typedef decltype(type) T;
@@ -634,11 +642,6 @@ inline void launch_group_norm(const GroupNormArgs &a, const GroupNormPlan &p, bo
       if (p.rows == 2) rows(nv, std::integral_constant<int, 2>(), lanes);
       else rows(nv, std::integral_constant<int, 1>(), lanes);
     };
-    auto slab = [&](auto nv) {
-      constexpr int NV = decltype(nv)::value;
-      if (p.aligned) launch_cluster_k(a.parts, group_norm_slab_kernel<T, true, NV>, dim3(p.grid, a.chunks), p.threads, p.smem, s, a);
-      else launch_cluster_k(a.parts, group_norm_slab_kernel<T, false, NV>, dim3(p.grid, a.chunks), p.threads, p.smem, s, a);
-    };
     auto by_nv = [&](auto use) {
       if (p.nv <= 1) use(std::integral_constant<int, 1>());
       else if (p.nv <= 2) use(std::integral_constant<int, 2>());
@@ -651,7 +654,10 @@ inline void launch_group_norm(const GroupNormArgs &a, const GroupNormPlan &p, bo
       else by_nv([&](auto nv) { by_rows(nv, std::integral_constant<int, 32>()); });
       break;
     case NORM_ROWS_BLOCK: by_nv([&](auto nv) { by_rows(nv, std::integral_constant<int, 0>()); }); break;
-    case NORM_SLAB: by_nv(slab); break;
+    case NORM_SLAB:
+      if (p.aligned) launch_cluster_k(a.parts, group_norm_slab_kernel<T, true>, dim3(p.grid, a.chunks), p.threads, p.smem, s, a);
+      else launch_cluster_k(a.parts, group_norm_slab_kernel<T, false>, dim3(p.grid, a.chunks), p.threads, p.smem, s, a);
+      break;
     case NORM_STREAMED: {
       auto both_passes = [&](auto aligned) {
         constexpr bool A = decltype(aligned)::value;

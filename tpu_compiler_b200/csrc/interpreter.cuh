@@ -1924,9 +1924,10 @@ public:
       p.err = &I.ss.d_err->code;
       p.wait_rounds = I.selftest_lost_arrival;
       p.lose_arrival = I.selftest_lost_arrival > 0;
-      encode_matrix_map(&tc_.tmX, (const int8_t *)in->dev, s.m, s.k_dev * 2, s.k_dev * 2, 128, l.pair ? 128 : l.a_rows);
-      encode_matrix_map(&tc_.tmW, (const int8_t *)w, out->cp, s.k_dev * 2, s.k_dev * 2, 128, l.pair ? l.nt / 2 : l.nt);
-      encode_matrix_map(&tc_.tmY, (const int8_t *)out->dev, s.m, out->cp * 2, out->cp * 2, 64, 32);
+      const int k_bytes = s.k_dev * 2, y_bytes = out->cp * 2;
+      encode_matrix_map(&tc_.tmX, (const int8_t *)in->dev, s.m, k_bytes, k_bytes, 128, l.pair ? 128 : l.a_rows);
+      encode_matrix_map(&tc_.tmW, (const int8_t *)w, out->cp, k_bytes, k_bytes, 128, l.pair ? l.nt / 2 : l.nt);
+      encode_matrix_map(&tc_.tmY, (const int8_t *)out->dev, s.m, y_bytes, y_bytes, 64, 32);
       linear_kernel_ready(tc_, act_);
     }
     alg_ops = 2.0 * s.m * k * s.n;
@@ -1936,6 +1937,7 @@ public:
     if (out_->dtype == DT_BF16) launch_linear_tc(tc_, act_, s);
     else launch_linear_f32(f32_, f32_plan_, s);
   }
+  bool is_tensor_core() const { return out_->dtype == DT_BF16; }
   std::string form() const override {
     if (out_->dtype != DT_BF16) return "tiles=direct rows=" + std::to_string(8 * f32_plan_.rm) + " split_k=" + std::to_string(f32_plan_.split);
     const LinearTcPlan &l = tc_.plan;
@@ -1965,6 +1967,8 @@ public:
     a_.eps = s.eps; a_.act = s.act;
     const int columns = plan_.vecs * (plan_.aligned ? 1 : 16 / (int)in->elsize());
     a_.lanes = plan_.lanes;
+    a_.held = plan_.nv;
+    group_norm_ready(plan_, out->dtype == DT_F32);
     a_.col_split = plan_.col_split;
     a_.group_span = plan_.group_span;
     a_.inv_group_width = 1.0f / (plan_.aligned ? a_.cg / (16 / (int)in->elsize()) : a_.cg);

@@ -146,14 +146,14 @@ inline GroupNormPlan group_norm_plan(int n, int pixels, int c, int groups, int e
     }
   }
   // chunks: whole groups and whole vectors; the smallest such unit, or the whole row
-  if (c >= 1 << 20 || (long long)n * 8 >= 1LL << 31) return p; // (small_div; the grid)
+  if (c >= 1 << 19 || (long long)n * 8 >= 1LL << 31) return p; // (small_div; the grid, 65535 chunks)
   int unit_groups = 1;
   while (unit_groups < groups && unit_groups * cg % N) ++unit_groups;
   const int unit_vecs = (unit_groups * cg + N - 1) / N;
   if (unit_vecs > 256) return p;
   const int units = (groups + unit_groups - 1) / unit_groups;
   auto lay_out = [&](int threads, int k, int parts) { // k units per chunk
-    k = std::max(1, std::min(k, std::min(units, threads / unit_vecs)));
+    k = std::max(1, std::min({k, units, threads / unit_vecs, 256 / unit_groups})); // (256 groups: shared memory of norm_group_sums, 45 KB)
     p.vecs = k * unit_vecs;
     p.chunk_groups = std::min(groups, k * unit_groups);
     p.chunks = (groups + p.chunk_groups - 1) / p.chunk_groups;
@@ -170,18 +170,31 @@ inline GroupNormPlan group_norm_plan(int n, int pixels, int c, int groups, int e
     p.group_span = round_up(p.col_split * group_width, 32);
     p.smem = ((size_t)threads * per + (size_t)p.chunk_groups * p.group_span / 32 * 33 + round_up(p.chunk_groups, 2)) * 4;
   };
-  // slab: 64 bytes of a pixel and more, at most 8 vectors per thread in at most eight blocks
+  // slab: 64 bytes of a pixel and more, in the shared memory of at most eight blocks. Few blocks are best, for the sums of each cost the same: at
+  // most six where fewer hold it (2 x 320 x 96 x 96 us with three modules in flight / alone: by four 7.7 / 18.5, six 9.0 / 16.4, eight 11.3 /
+  // 22.6, streamed 11.6 / 22.6). Where a block leaves no room for a second one on its SM, nothing fills the time of its loads and sums: then only if
+  // they run at once and on half of the SMs, else by more blocks (16 x 256 x 64 x 64 by two 17.8 / 22.6, by three 16.3 / 22.3, streamed 18.8 / 28.5;
+  // 6 x 62 x 100 x 100 by seven 6.2 / 16.4, streamed 6.1 / 12.3).
   const int wide = (4 + unit_vecs - 1) / unit_vecs;
   lay_out(kSlabThreads, wide, 1);
-  const int lanes = kSlabThreads / p.vecs, need = (pixels + 8 * lanes - 1) / (8 * lanes);
-  if (need <= 8 && mode != 1 + NORM_STREAMED && p.smem + (size_t)p.chunk_groups * 16 <= 48 * 1024) { // (shared memory that a kernel has unasked)
-    int parts = need;
-    while (parts < 8 && (long long)n * p.chunks * parts <= sm_count && pixels > 2 * parts * lanes) parts *= 2;
-    lay_out(kSlabThreads, wide, std::min(parts, 8));
-    p.form = NORM_SLAB;
-    p.smem += (size_t)p.chunk_groups * 16;
-    // ... where its blocks all run at once
-    if (mode == 1 + NORM_SLAB || (long long)p.grid * p.chunks <= (p.nv <= 4 ? 2LL : 1LL) * sm_count) return p;
+  if (mode != 1 + NORM_STREAMED) {
+    const size_t fixed = p.smem + (size_t)p.chunk_groups * 16, half = 113 * 1024;
+    const long long slabs = (long long)n * p.chunks, lanes = p.lanes;
+    auto parts_in = [&](size_t room) { // 9: none do
+      const long long held = fixed < room ? (long long)((room - fixed) / (kSlabThreads * 16)) : 0;
+      return held ? (int)std::min(9LL, (pixels + held * lanes - 1) / (held * lanes)) : 9;
+    };
+    auto try_slab = [&](int parts) {
+      if (parts > 8) return false;
+      lay_out(kSlabThreads, wide, parts);
+      p.smem = fixed + (size_t)p.nv * kSlabThreads * 16;
+      p.form = NORM_SLAB;
+      return p.smem <= half || (slabs * p.parts <= sm_count && 2 * slabs * p.parts >= sm_count);
+    };
+    const int need = parts_in(2 * half);
+    const long long spread = std::min({6LL, sm_count / slabs, (pixels + 2 * lanes - 1) / (2 * lanes)});
+    if (try_slab((int)std::max<long long>(need, spread)) || try_slab(parts_in(half)) || (mode == 1 + NORM_SLAB && need <= 8)) return p;
+    p.form = NORM_STRIDED;
   }
   // streamed: chunks of whole rows where they fit, and as many parts of the image as run at once; a thread has 8 vectors at least
   const int most_units = std::max(1, 256 / unit_vecs);
