@@ -526,3 +526,17 @@ def test_refusals_reach_the_caller(M):
     m.invoke()
     assert (m.get_tensor("y") == 0).all()
     m.close()
+
+
+@pytest.mark.parametrize("dtype,bound", [("BF16", "tensor"), ("FP32", "hbm")])
+def test_op_info(M, dtype, bound):
+    """What a module says of these ops to who accounts for its time."""
+    m = M(0)
+    m.load_text("input name=x shape=4,64 dtype=%s\ngroup_norm name=z in=x shape=4,64 dtype=%s groups=1\n"
+                "fully_connected name=y in=z,f shape=4,32 dtype=%s activation=silu\n" % (dtype, dtype, dtype),
+                {"f": np.ones((32, 64), np.float32)})
+    z, y = [i for i in m.op_info if i["name"] in ("y", "z")][:2]
+    size = 2 if dtype == "BF16" else 4
+    assert (z["type"], z["bound"], z["bytes"]) == ("group_norm", "hbm", 2 * 4 * 64 * size + 8 * 64)
+    assert (y["type"], y["bound"], y["ops"]) == ("fully_connected", bound, 2 * 4 * 64 * 32)
+    m.close()

@@ -365,7 +365,8 @@ int tpucb_interp_get_op_info(tpucb_interp *it, char *out, size_t cap, size_t *ne
     s += "\t" + std::to_string(k->alg_ops) + "\t" + std::to_string(k->alg_bytes);
     auto *cv = dynamic_cast<Conv2DOp *>(k.get());
     auto *fc = dynamic_cast<FullyConnectedOp *>(k.get());
-    s += std::string("\t") + ((cv && cv->is_tensor_core()) || (fc && !fc->is_batched()) ? "tensor" : "hbm") + "\n";
+    auto *li = dynamic_cast<LinearOp *>(k.get());
+    s += std::string("\t") + ((cv && cv->is_tensor_core()) || (fc && !fc->is_batched()) || (li && li->is_tensor_core()) ? "tensor" : "hbm") + "\n";
   }
   copy_out(s, out, cap, needed);
   TPUCB_API_END
