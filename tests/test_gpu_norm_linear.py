@@ -540,3 +540,22 @@ def test_op_info(M, dtype, bound):
     assert (z["type"], z["bound"], z["bytes"]) == ("group_norm", "hbm", 2 * 4 * 64 * size + 8 * 64)
     assert (y["type"], y["bound"], y["ops"]) == ("fully_connected", bound, 2 * 4 * 64 * 32)
     m.close()
+
+
+@pytest.mark.parametrize("dtype,n,tiles", [("BF16", 20, 1), ("BF16", 20, 4032), ("BF16", 200, 10064), ("BF16", 37, 10128), ("BF16", 17, 1128), ("FP32", 18, 1), ("FP32", 21, 2008)])
+def test_linear_infinities_stay_infinities(M, dtype, n, tiles):
+    """An infinite value of a row gives infinite sums, in the next product too: what lies behind the last channel adds no NaN to them."""
+    rng = np.random.default_rng(41)
+    x = cast(rng.uniform(1, 2, (300, 48)), dtype)
+    x[1, 3] = np.inf
+    f, f2 = (cast(rng.uniform(0.5, 1, s), dtype) for s in ((n, 48), (9, n)))
+    m = M(0)
+    m.set_option("linear_tiles", tiles)
+    m.load_text("input name=x shape=300,48 dtype=%s\nfully_connected name=h in=x,f shape=300,%d dtype=%s activation=relu\n"
+                "fully_connected name=y in=h,f2 shape=300,9 dtype=%s activation=silu\n" % (dtype, n, dtype, dtype), {"f": f, "f2": f2})
+    m.set_tensor("x", x)
+    m.invoke()
+    for name in ("h", "y"):
+        got = m.get_tensor(name)
+        assert np.isposinf(got[1]).all() and np.isfinite(np.delete(got, 1, 0)).all()
+    m.close()

@@ -1909,13 +1909,13 @@ public:
     if (out->dtype == DT_F32) {
       f32_plan_ = linear_f32_plan(s.m, s.k_dev, out->cp, I.sm_count, I.linear_tiles);
       f32_ = LinearF32Args{(const float *)in->dev, (const float *)w, res_ ? (const float *)res_->dev : nullptr, bias, (float *)out->dev,
-                           s.m, s.k_dev, out->cp, out->cp, f32_plan_.split, s.act};
+                           s.m, s.k_dev, s.n, out->cp, out->cp, f32_plan_.split, s.act};
     }
     if (out->dtype == DT_BF16) {
       const LinearTcPlan &l = tc_.plan = linear_tc_plan(s.m, s.k_dev, out->cp, I.sm_count, I.linear_tiles);
       LinearTcParams &p = tc_.p;
       p = LinearTcParams{};
-      p.m = s.m; p.n_pad = p.ldy = out->cp;
+      p.m = s.m; p.n = s.n; p.n_pad = p.ldy = out->cp;
       p.k_blocks = l.k_blocks; p.nt = l.nt; p.split = l.split; p.a_rows = l.a_rows; p.stages = l.stages; p.tmem_cols = l.tmem_cols;
       p.idesc = make_idesc_bf16(l.pair ? 256 : 128, l.nt);
       p.bias = bias;
@@ -1924,10 +1924,10 @@ public:
       p.err = &I.ss.d_err->code;
       p.wait_rounds = I.selftest_lost_arrival;
       p.lose_arrival = I.selftest_lost_arrival > 0;
-      const int k_bytes = s.k_dev * 2, y_bytes = out->cp * 2;
+      const int k_bytes = s.k_dev * 2;
       encode_matrix_map(&tc_.tmX, (const int8_t *)in->dev, s.m, k_bytes, k_bytes, 128, l.pair ? 128 : l.a_rows);
       encode_matrix_map(&tc_.tmW, (const int8_t *)w, out->cp, k_bytes, k_bytes, 128, l.pair ? l.nt / 2 : l.nt);
-      encode_matrix_map(&tc_.tmY, (const int8_t *)out->dev, s.m, y_bytes, y_bytes, 64, 32);
+      encode_matrix_map(&tc_.tmY, (const int8_t *)out->dev, s.m, out->cp * 2, out->cp * 2, 64, 32);
       linear_kernel_ready(tc_, act_);
     }
     alg_ops = 2.0 * s.m * k * s.n;

@@ -17,7 +17,7 @@ struct LinearF32Args {
   const float *x, *w, *res; // [m][k], [n_pad][k], null or [m][ldy]
   const float *bias;        // [n_pad]
   float *y;                 // [m][ldy]
-  int m, k, n_pad, ldy;     // k and ldy with the padding of the channel pitch (multiples of 4), whose weights and bias are zero
+  int m, k, n, n_pad, ldy;  // k, n_pad and ldy with the padding of the channel pitch (multiples of 4), whose weights and bias are zero
   int split, act;
 };
 
@@ -147,7 +147,9 @@ template <int RM> __global__ void __launch_bounds__(kF32Threads, 4) linear_f32_k
         v0 = v0 + Pair(r.x, r.y);
         v1 = v1 + Pair(r.z, r.w);
       }
-      *reinterpret_cast<float4 *>(a.y + o) = make_float4(v0.lo(), v0.hi(), v1.lo(), v1.hi());
+      // (padded channels stay zero: an infinity of x times their weights is a NaN)
+      const int valid = a.n - n0 - col;
+      *reinterpret_cast<float4 *>(a.y + o) = make_float4(v0.lo(), valid > 1 ? v0.hi() : 0.0f, valid > 2 ? v1.lo() : 0.0f, valid > 3 ? v1.hi() : 0.0f);
     }
   });
   __syncwarp();

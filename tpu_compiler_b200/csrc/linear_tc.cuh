@@ -24,7 +24,7 @@ namespace tpucb {
 
 // (its sizes: linear_tc_plan)
 struct LinearTcParams {
-  int m, n_pad;   // rows; channels with the padding of the pitch, whose weights and bias are zero
+  int m, n, n_pad; // rows; channels, without and with the padding of the pitch, whose weights and bias are zero
   int ldy;        // pitch of y and the residual, in values
   int k_blocks;   // of 64 values
   int nt;         // channels per tile: a multiple of 16 (pair: of 64), at most 256
@@ -70,7 +70,9 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
 }
 } // namespace ptx
 
-// Sixteen channels of one row: bias, activation, residual, rounding.
+// Sixteen channels of one row: bias, activation, residual, rounding. Padded channels become zero whatever is in x: an infinity times their zero
+// weights would be a NaN, which the next inner product would add to its sums. (A map that ends with the channels does not keep the bulk stores from
+// them: they write 16 bytes at a time.)
 template <int ACT> __device__ __forceinline__ void linear_finish16(const uint32_t *acc, const LinearTcParams &p, size_t at, int col, uint32_t (&o)[8]) {
   uint32_t r[8];
   const bool residual = p.res && col < p.n_pad;
@@ -86,6 +88,10 @@ template <int ACT> __device__ __forceinline__ void linear_finish16(const uint32_
       if (residual) v[j] = v[j] + pair_of_bf16(r[2 * q + j]);
       o[2 * q + j] = bf16x2_ieee(v[j].lo(), v[j].hi());
     }
+  }
+  if (col + 16 > p.n) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] &= (col + 2 * j < p.n ? 0xffffu : 0u) | (col + 2 * j + 1 < p.n ? 0xffff0000u : 0u);
   }
 }
 template <int ACT> __device__ __forceinline__ void linear_store16(const uint32_t *acc, const LinearTcParams &p, int row, int col) {
@@ -413,7 +419,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
               uint32_t o[8];
-              // (columns behind the last are clipped by the map; there is bias for them, and no residual)
+              // (columns behind the pitch are clipped by the map; there is bias for them, and no residual)
               linear_finish16<ACT>(r + 16 * q, p, (size_t)(m0 + row) * p.ldy + n0 + c + 16 * q, n0 + c + 16 * q, o);
               // the map's 64-byte swizzle: a row's piece i of 16 bytes lies at i ^ (row / 2 % 4)
 #pragma unroll
