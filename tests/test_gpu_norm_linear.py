@@ -143,6 +143,7 @@ def test_group_norm_forms(M, form, shape, groups, dtype):
 @pytest.mark.parametrize("dtype", ["BF16", "FP32"])
 @pytest.mark.parametrize("form,shape,groups", [
     ("slab", (1, 320, 96, 100), 32), ("slab", (1, 96, 70, 111), 8), ("slab", (2, 64, 90, 90), 2), ("slab", (150, 64, 20, 20), 32),  # most of shared memory
+    ("slab", (2, 1500, 9, 9), 1),  # wide groups
     ("streamed", (1, 512, 40, 60), 512), ("streamed", (1, 2048, 20, 21), 2048), ("streamed", (1, 2100, 20, 21), 300),  # many groups per row
     ("strided", (1, 524400, 2, 1), 8)])  # more channels than the others divide
 def test_group_norm_at_its_limits(M, form, shape, groups, dtype):

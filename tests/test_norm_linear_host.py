@@ -76,7 +76,7 @@ def checks(tmp_path_factory):
 
 
 NORM_IN = ["w g 48", "w b 48", "w short 47", "input name=x shape=2,48,5,3 dtype=BF16", "input name=q shape=2,48,5,3 dtype=INT8",
-           "input name=none shape=0,48 dtype=BF16"]
+           "input name=none shape=0,48 dtype=BF16", "input name=wide shape=1,1,32768,32768 dtype=BF16"]
 
 
 @pytest.mark.parametrize("line,answer", [
@@ -98,6 +98,7 @@ NORM_IN = ["w g 48", "w b 48", "w short 47", "input name=x shape=2,48,5,3 dtype=
     ("group_norm name=y in=x,short,b shape=2,48,5,3 dtype=BF16 groups=4", "47 values, expected 48"),
     ("group_norm name=y in=x,g,lost shape=2,48,5,3 dtype=BF16 groups=4", "was not registered"),
     ("group_norm name=y in=none,-,- shape=0,48 dtype=BF16 groups=4", "empty tensor"),
+    ("group_norm name=y in=wide shape=1,1,32768,32768 dtype=BF16 groups=1", "too many pixels"),
 ])
 def test_group_norm_arguments(checks, line, answer):
     got, = checks(NORM_IN + [line])
@@ -196,7 +197,10 @@ int norm(int n, int pixels, int c, int groups, int es, int sms, int mode) {
       EXPECT((long long)p.apply_parts * p.apply_pixels >= pixels && (long long)(p.apply_parts - 1) * p.apply_pixels < pixels);
       EXPECT(p.apply_grid == (unsigned)(n * p.apply_parts) && p.apply_pixels <= 1 << 22);
     }
-  } else EXPECT(p.grid == (unsigned)(n * groups));
+  } else {
+    EXPECT(p.parts <= (int)p.threads && p.grid == (unsigned)(n * groups * p.parts) && (long long)n * groups * p.parts < 1LL << 31);
+    EXPECT(p.part_values * p.parts >= (long long)pixels * cg && p.part_values * (p.parts - 1) < (long long)pixels * cg);
+  }
   return 0;
 }
 int linear(int m, int k, int n, int sms, int mode) {

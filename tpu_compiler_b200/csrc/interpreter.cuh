@@ -1974,16 +1974,15 @@ public:
     a_.inv_group_width = 1.0f / (plan_.aligned ? a_.cg / (16 / (int)in->elsize()) : a_.cg);
     a_.inv_vecs = 1.0f / plan_.vecs; a_.inv_lanes = 1.0f / plan_.lanes; a_.inv_cg = 1.0f / a_.cg; a_.inv_width = 1.0f / columns;
     a_.vecs = plan_.vecs; a_.chunk_groups = plan_.chunk_groups; a_.chunks = plan_.chunks; a_.parts = plan_.parts; a_.part_pixels = plan_.part_pixels;
-    if (plan_.form == NORM_STREAMED) {
-      a_.apply_parts = plan_.apply_parts;
-      a_.apply_pixels = plan_.apply_pixels;
-      a_.partial = (float2 *)I.dalloc((size_t)in->n * s.groups * plan_.parts * sizeof(float2));
-    }
+    a_.apply_parts = plan_.apply_parts;
+    a_.apply_pixels = plan_.apply_pixels;
+    a_.part_values = plan_.part_values;
+    if (kernel_launches() == 2) a_.partial = (float2 *)I.dalloc((size_t)in->n * s.groups * plan_.parts * sizeof(float2));
     alg_ops = 8.0 * in->numel();
     alg_bytes = 2.0 * in->numel() * in->elsize() + 8.0 * in->c;
   }
   void invoke(cudaStream_t s) override { launch_group_norm(a_, plan_, out_->dtype == DT_F32, s); }
-  int kernel_launches() const override { return plan_.form == NORM_STREAMED ? 2 : 1; }
+  int kernel_launches() const override { return plan_.form == NORM_STREAMED || plan_.form == NORM_STRIDED ? 2 : 1; }
   std::string form() const override {
     static const char *names[] = {"rows_warp", "rows_block", "slab", "streamed", "strided"};
     return std::string("form=") + names[plan_.form] + " parts=" + std::to_string(plan_.parts);

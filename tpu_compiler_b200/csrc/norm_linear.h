@@ -39,7 +39,7 @@ inline GroupNormSpec group_norm_spec(const ParsedOp &op, const DevTensor &in, co
   s.eps = (float)op.getf("variance_epsilon", 1e-5);
   TPUCB_CHECK(s.eps > 0.0f && std::isfinite(s.eps), "group_norm %s: variance_epsilon must be a positive fp32 number", nm);
   s.act = activation_from_string(op.gets("activation", "none"), "group_norm " + op.name);
-  TPUCB_CHECK((double)in.h * in.w < 2147483648.0 && (double)in.n * s.groups < 2147483648.0, "group_norm %s: too many pixels or groups", nm);
+  TPUCB_CHECK((double)in.h * in.w < (double)(1 << 30) && (double)in.n * s.groups < 2147483648.0, "group_norm %s: too many pixels or groups", nm);
   auto affine = [&](size_t i, float absent) {
     std::vector<float> v(in.cp, 0.0f);
     std::fill(v.begin(), v.begin() + in.c, absent);
@@ -110,15 +110,22 @@ struct GroupNormPlan {
   int col_split = 1, group_span = 32;
   int apply_parts = 1, apply_pixels = 0;
   unsigned apply_grid = 0;
+  long long part_values = 0; // strided: of a group, per block
   size_t smem = 0;
 };
 // mode (option "norm_form"): 0 by size, else 1 + the form, where it can
 inline GroupNormPlan group_norm_plan(int n, int pixels, int c, int groups, int es, int sm_count, int mode) {
   const int N = 16 / es, cg = c / groups;
   GroupNormPlan p;
-  p.grid = (unsigned)(n * groups);
   p.aligned = cg % N == 0;
-  if (mode == 1 + NORM_STRIDED) return p;
+  // strided: as many parts of a group as run at once, 2048 values or more each
+  const long long values = (long long)pixels * cg, lots = (long long)n * groups;
+  p.parts = (int)std::max(1LL, std::min({256LL, 8LL * sm_count / lots, values / 2048}));
+  p.part_values = (values + p.parts - 1) / p.parts;
+  p.parts = (int)((values + p.part_values - 1) / p.part_values);
+  p.grid = (unsigned)(lots * p.parts);
+  const GroupNormPlan strided = p;
+  if (mode == 1 + NORM_STRIDED) return strided;
   if (pixels == 1 && (p.aligned || groups == 1) && mode <= 1 + NORM_ROWS_BLOCK) {
     // a thread keeps up to 8 vectors: 8 lanes of a warp, a warp, or a block, which is larger where there are too few rows for all SMs
     const int nvec = (cg + N - 1) / N;
@@ -131,6 +138,7 @@ inline GroupNormPlan group_norm_plan(int n, int pixels, int c, int groups, int e
     };
     if (nvec <= 8 * 32 && mode != 1 + NORM_ROWS_BLOCK) {
       p.form = NORM_ROWS_WARP;
+      p.parts = 1;
       p.threads = 128;
       p.lanes = nvec <= 16 ? 8 : 32;
       const int per_block = 128 / p.lanes;
@@ -139,6 +147,7 @@ inline GroupNormPlan group_norm_plan(int n, int pixels, int c, int groups, int e
     }
     if (nvec <= 8 * 512) {
       p.form = NORM_ROWS_BLOCK;
+      p.parts = 1;
       const int want = many ? 4 : 2;
       p.threads = (unsigned)std::max(64, std::min(512, round_up((nvec + want - 1) / want, 32)));
       p.grid = (unsigned)units((int)p.threads);
@@ -146,11 +155,11 @@ inline GroupNormPlan group_norm_plan(int n, int pixels, int c, int groups, int e
     }
   }
   // chunks: whole groups and whole vectors; the smallest such unit, or the whole row
-  if (c >= 1 << 19 || (long long)n * 8 >= 1LL << 31) return p; // (small_div; the grid, 65535 chunks)
+  if (c >= 1 << 19 || (long long)n * 8 >= 1LL << 31) return strided; // (small_div; the grid, 65535 chunks)
   int unit_groups = 1;
   while (unit_groups < groups && unit_groups * cg % N) ++unit_groups;
   const int unit_vecs = (unit_groups * cg + N - 1) / N;
-  if (unit_vecs > 256) return p;
+  if (unit_vecs > kSlabThreads) return strided;
   const int units = (groups + unit_groups - 1) / unit_groups;
   auto lay_out = [&](int threads, int k, int parts) { // k units per chunk
     k = std::max(1, std::min({k, units, threads / unit_vecs, 256 / unit_groups})); // (256 groups: shared memory of norm_group_sums, 45 KB)
@@ -194,8 +203,8 @@ inline GroupNormPlan group_norm_plan(int n, int pixels, int c, int groups, int e
     const int need = parts_in(2 * half);
     const long long spread = std::min({6LL, sm_count / slabs, (pixels + 2 * lanes - 1) / (2 * lanes)});
     if (try_slab((int)std::max<long long>(need, spread)) || try_slab(parts_in(half)) || (mode == 1 + NORM_SLAB && need <= 8)) return p;
-    p.form = NORM_STRIDED;
   }
+  if (unit_vecs > kStreamThreads) return strided;
   // streamed: chunks of whole rows where they fit, and as many parts of the image as run at once; a thread has 8 vectors at least
   const int most_units = std::max(1, 256 / unit_vecs);
   lay_out(kStreamThreads, most_units, 1);
