@@ -63,6 +63,7 @@ __device__ __forceinline__ void tcgen05_ld_x32(uint32_t taddr, uint32_t (&r)[32]
       : "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void prefetch_l2(const void *p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p) : "memory"); }
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
@@ -135,103 +136,99 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
   const uint32_t b_at = (a_bytes + 1023u) & ~1023u, stage_bytes = b_at + ((b_bytes + 1023u) & ~1023u);
   const int wait_rounds = p.wait_rounds > 0 ? p.wait_rounds : 1024;
 
+  const int ahead = min(nk, p.stages);
   if (threadIdx.x == 0) {
-    const int gave_up = *reinterpret_cast<volatile int *>(p.err);
     for (int s = 0; s < p.stages; ++s) {
       ptx::mbar_init(bar_full + 8 * s, 2); // weights, rows
       ptx::mbar_init(bar_empty + 8 * s, 1);
     }
     ptx::mbar_init(bar_acc, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    *abort_flag = gave_up;
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    *abort_flag = 0;
+    // weights are written at load time only: they need not wait for the previous kernel, nor for the other warps
+    for (int i = 0; i < ahead; ++i) {
+      ptx::mbar_expect_tx(bar_full + 8 * i, b_bytes);
+      ptx::tma_load_2d(ring + (uint32_t)i * stage_bytes + b_at, &tmW, bar_full + 8 * i, (kb0 + i) * 128, n0);
+    }
   }
+  if (threadIdx.x == 64) asm volatile("prefetch.tensormap [%0];" ::"l"(&tmX) : "memory");
   if (warp == 1) ptx::tcgen05_alloc(ptx::smem_u32(tmem_slot), p.tmem_cols);
   ptx::tcgen05_fence_before();
   __syncthreads();
   ptx::tcgen05_fence_after();
   pdl_trigger(); // (behind the allocation: a successor's CTA on this SM does not take what this one needs)
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-  bool ok = *abort_flag == 0;
+  bool ok = true;
 
   if (warp == 0) {
-    if (ok) {
-      const int ahead = min(nk, p.stages);
+    pdl_wait();
+    if (ptx::elect_one()) {
+      for (int i = 0; i < ahead; ++i) {
+        ptx::mbar_expect_tx(bar_full + 8 * i, a_bytes);
+        ptx::tma_load_2d(ring + (uint32_t)i * stage_bytes, &tmX, bar_full + 8 * i, (kb0 + i) * 128, m0);
+      }
+    }
+    __syncwarp();
+    int s = 0;
+    uint32_t ph = 0;
+    for (int i = ahead; i < nk; ++i) {
+      if (!ptx::mbar_wait_warp(bar_empty + 8 * s, ph, abort_flag, wait_rounds)) {
+        wait_expired(p.err, abort_flag, kErrEmptyWait);
+        break;
+      }
       if (ptx::elect_one()) {
-        for (int i = 0; i < ahead; ++i) { // weights are written at load time only: they need not wait for the previous kernel
-          ptx::mbar_expect_tx(bar_full + 8 * i, b_bytes);
-          ptx::tma_load_2d(ring + (uint32_t)i * stage_bytes + b_at, &tmW, bar_full + 8 * i, (kb0 + i) * 128, n0);
-        }
+        const uint32_t at = ring + (uint32_t)s * stage_bytes, fb = bar_full + 8 * s;
+        ptx::mbar_expect_tx(fb, b_bytes);
+        ptx::tma_load_2d(at + b_at, &tmW, fb, (kb0 + i) * 128, n0);
+        ptx::mbar_expect_tx(fb, a_bytes);
+        ptx::tma_load_2d(at, &tmX, fb, (kb0 + i) * 128, m0);
       }
-      __syncwarp();
-      pdl_wait();
-      if (ptx::elect_one()) {
-        for (int i = 0; i < ahead; ++i) {
-          ptx::mbar_expect_tx(bar_full + 8 * i, a_bytes);
-          ptx::tma_load_2d(ring + (uint32_t)i * stage_bytes, &tmX, bar_full + 8 * i, (kb0 + i) * 128, m0);
-        }
+      if (++s == p.stages) {
+        s = 0;
+        ph ^= 1u;
       }
-      __syncwarp();
-      int s = 0;
-      uint32_t ph = 0;
-      for (int i = ahead; i < nk; ++i) {
-        if (!ptx::mbar_wait_warp(bar_empty + 8 * s, ph, abort_flag, wait_rounds)) {
-          wait_expired(p.err, abort_flag, kErrEmptyWait);
-          ok = false;
-          break;
-        }
-        if (ptx::elect_one()) {
-          const uint32_t at = ring + (uint32_t)s * stage_bytes, fb = bar_full + 8 * s;
-          ptx::mbar_expect_tx(fb, b_bytes);
-          ptx::tma_load_2d(at + b_at, &tmW, fb, (kb0 + i) * 128, n0);
-          ptx::mbar_expect_tx(fb, a_bytes);
-          ptx::tma_load_2d(at, &tmX, fb, (kb0 + i) * 128, m0);
-        }
-        if (++s == p.stages) {
-          s = 0;
-          ph ^= 1u;
-        }
-      }
-      if (!ok || *abort_flag) drain_copies();
     }
   } else if (warp == 1) {
-    if (ok) {
-      const uint64_t desc0 = make_kmajor_desc(ring, 128);
-      const uint32_t hi = (uint32_t)(desc0 >> 32), lo0 = (uint32_t)desc0, step = stage_bytes >> 4, w_at = b_at >> 4;
-      int s = 0;
-      uint32_t ph = 0, lo = lo0;
-      for (int i = 0; i < nk; ++i) {
-        if (!ptx::mbar_wait_warp(bar_full + 8 * s, ph, abort_flag, wait_rounds)) {
-          wait_expired(p.err, abort_flag, kErrFullWait);
-          ok = false;
-          break;
-        }
-        ptx::tcgen05_fence_after();
-        if (ptx::elect_one()) {
-          ptx::tcgen05_mma_i8_kblock<4, 1>(tmem, lo, lo + w_at, hi, p.idesc, i > 0 ? 1u : 0u);
-          ptx::tcgen05_commit(bar_empty + 8 * s);
-        }
-        lo += step;
-        if (++s == p.stages) {
-          s = 0;
-          ph ^= 1u;
-          lo = lo0;
-        }
+    const uint64_t desc0 = make_kmajor_desc(ring, 128);
+    const uint32_t hi = (uint32_t)(desc0 >> 32), lo0 = (uint32_t)desc0, step = stage_bytes >> 4, w_at = b_at >> 4;
+    int s = 0;
+    uint32_t ph = 0, lo = lo0;
+    for (int i = 0; i < nk; ++i) {
+      if (!ptx::mbar_wait_warp(bar_full + 8 * s, ph, abort_flag, wait_rounds)) {
+        wait_expired(p.err, abort_flag, kErrFullWait);
+        ok = false;
+        break;
       }
-      if (ok && !p.lose_arrival && ptx::elect_one()) ptx::tcgen05_commit(bar_acc);
-      __syncwarp();
+      ptx::tcgen05_fence_after();
+      if (ptx::elect_one()) {
+        ptx::tcgen05_mma_i8_kblock<4, 1>(tmem, lo, lo + w_at, hi, p.idesc, i > 0 ? 1u : 0u);
+        ptx::tcgen05_commit(bar_empty + 8 * s);
+      }
+      lo += step;
+      if (++s == p.stages) {
+        s = 0;
+        ph ^= 1u;
+        lo = lo0;
+      }
     }
+    if (ok && !p.lose_arrival && ptx::elect_one()) ptx::tcgen05_commit(bar_acc);
+    __syncwarp();
   } else {
+    const int cols = min(p.nt, p.n_pad - n0);
+    if (lane * 32 < cols) ptx::prefetch_l2(p.bias + n0 + lane * 32);
     pdl_wait(); // the residual
-    if (ok) {
-      ok = __all_sync(0xffffffffu, ptx::mbar_wait_bounded(bar_acc, 0, abort_flag, wait_rounds));
-      if (!ok) wait_expired(p.err, abort_flag, kErrAccWait);
-    }
+    // a kernel that gave up earlier ends this one's waits
+    if (threadIdx.x == 64 && *reinterpret_cast<volatile int *>(p.err) != 0) *abort_flag = 1;
+    if (p.res && m0 + (warp & 3) * 32 + lane < p.m)
+      for (int c = rank * 64; c < cols; c += p.split * 64) ptx::prefetch_l2(p.res + (size_t)(m0 + (warp & 3) * 32 + lane) * p.ldy + n0 + c);
+    ok = __all_sync(0xffffffffu, ptx::mbar_wait_bounded(bar_acc, 0, abort_flag, wait_rounds));
+    if (!ok) wait_expired(p.err, abort_flag, kErrAccWait);
     ptx::tcgen05_fence_after();
     const int quarter = warp & 3, row = quarter * 32 + lane;
     const int rows = min(128, (p.m - m0 + 31) & ~31); // of the partial sums that are exchanged
     if (ok && quarter * 32 < rows) {
       const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16);
-      const int cols = min(p.nt, p.n_pad - n0);
       for (int c = 0; c < cols; c += 16) {
         uint32_t r[16];
         ptx::tcgen05_ld_x16(acc + (uint32_t)c, r);
@@ -251,6 +248,7 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
   ptx::tcgen05_fence_before();
   __syncthreads();
   if (warp == 1) {
+    if (*abort_flag) drain_copies();
     ptx::tcgen05_fence_after();
     ptx::tcgen05_dealloc(tmem, p.tmem_cols);
   }
