@@ -159,6 +159,17 @@ def test_oracle_definitions_against_torch(act):
     assert np.abs(O.linear64(rows, w, bias, act, r) - want).max() < 2 ** -45 * 64
 
 
+@pytest.mark.parametrize("line", ["group_norm name=y in=x shape=2,16 dtype=FP32 groups=1",
+                                  "fully_connected name=y in=x,f,b shape=2,16 dtype=FP32 activation=gelu",
+                                  "fully_connected name=y in=x,f,b,-,-,-,-,x shape=2,16 dtype=FP32"])
+def test_int8_quantisation_refuses(line):
+    """Neither op has an INT8 form: an fp32 graph with one is not quantised into one without it."""
+    from tpu_compiler_b200 import quantize
+    weights = {"f": np.ones((16, 16), np.float32), "b": np.ones(16, np.float32)}
+    with pytest.raises(NotImplementedError, match="is not covered"):
+        quantize.quantize_module("input name=x shape=2,16 dtype=FP32\n" + line + "\n", weights, {"x": 1.0, "y": 2.0})
+
+
 PLANS = r"""
 #include "norm_linear.h"
 #include <iostream>

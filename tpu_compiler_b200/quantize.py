@@ -371,6 +371,8 @@ def quantize_op(op, thr, weights, by_name, rename=None, out_name=None, cache=Non
             new["in"][2] = name + "_bias_q"
         w[name + "_rshift"], w[name + "_multiplier"] = r, m
     elif t == "fully_connected":
+        if "activation" in op["attrs"] or (len(op["in"]) > 7 and op["in"][7]):
+            raise NotImplementedError("quantize: op type fully_connected with activation or residual (%s) is not covered" % op["name"])
         bias = weights[op["in"][2]] if len(op["in"]) > 2 and op["in"][2] else None
         nf, nb, r, m = quantize_fc_weights(weights[op["in"][1]], bias, ty, txs[0])
         w[name + "_filter_q"] = nf
