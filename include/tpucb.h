@@ -58,7 +58,19 @@ int tpucb_interp_set_weight(tpucb_interp *it, const char *name, const float *dat
  *     <op_type> name=<result> in=<operand>,<operand>,... shape=<d0>,<d1>,.. dtype=INT8|BF16|FP32 key=value ...
  * with the operand order of the TPU dialect op ("-" for an absent operand) and the
  * attribute names of the dialect's param structs. An op the backend does not implement
- * is an error here, not at run time. */
+ * is an error here, not at run time.
+ * Two forms without a reference counterpart, for the blocks of transformer and diffusion graphs, both for BF16 and FP32 tensors (an INT8 graph
+ * runs them between quant ops):
+ *     group_norm name=y in=x,<gamma|->,<beta|-> shape=.. dtype=.. groups=G variance_epsilon=1e-5 activation=none|relu|silu|gelu|gelu_tanh
+ * y = act((x - mean) / sqrt(var + variance_epsilon) gamma + beta), mean and biased variance over the pixels of an image and the c / G
+ * channels of a group; G must divide c, x and y have one shape and type, gamma and beta c values each (absent: 1 and 0). G = 1 on a
+ * [tokens, channels] tensor is layer norm.
+ *     fully_connected name=y in=x,filter,<bias|->,-,-,-,-,<residual|-> shape=m,n dtype=.. activation=none|relu|silu|gelu|gelu_tanh
+ * y = act(x filter^T + bias) + residual: a fully_connected line that names an activation or an operand 7 (a tensor of y's shape and type).
+ * do_relu=1 beside a residual is activation=relu; both attributes at once are refused, and so are filters of rank 3. gelu is
+ * x Phi(x), gelu_tanh its approximation by tanh. BF16 results of these two are rounded to nearest even, infinities and NaN kept, sums,
+ * statistics and activations are fp32; a NaN or an infinity stays within its group or row. The order of sums depends on the shapes,
+ * the options and the GPU's number of SMs alone: a module gives the same bits every time. */
 int tpucb_interp_load_module(tpucb_interp *it, const char *module_text);
 
 /* MlirModuleInterpreter::setTensor (MlirModuleInterpreter.cpp:407-417). */
@@ -137,7 +149,9 @@ int tpucb_interp_get_details(tpucb_interp *it, int outputs, char *out, size_t ca
 int tpucb_interp_get_op_info(tpucb_interp *it, char *out, size_t cap, size_t *needed);
 /* How the rules by size, type and value range run a convolution or an inner product (no reference counterpart), as "key=value" words:
  * tiles (small, big, stem; depthwise; direct), and for the tensor-core forms ctas and pixels per tile, split_k (CTAs that share a
- * tile's K), requant (float, integer: a high multiply, wide: 64-bit; none outside INT8). Empty for other ops. */
+ * tile's K), requant (float, integer: a high multiply, wide: 64-bit; none outside INT8). For inner products with activation or residual: tiles
+ * (cluster, pair: of two SMs; direct: fp32), channels or (fp32) rows per tile, split_k. For group_norm: form (rows_warp, rows_block, slab,
+ * streamed, strided), parts (blocks per image or group). Empty for other ops. */
 int tpucb_interp_get_op_form(tpucb_interp *it, const char *name, char *out, size_t cap, size_t *needed);
 
 /* Options: "cuda_graph" (0/1, default 1): replay the op list as one CUDA graph.
@@ -153,6 +167,11 @@ int tpucb_interp_get_op_form(tpucb_interp *it, const char *name, char *out, size
  *          "big_tiles" (0 never, 1 = default: by size, else 1000 * CTAs (1, 2) + pixels (32 .. 256, a multiple of 32): every
  *          layer that can, in this form; read by the next load_module): tensor-core convolutions that fill the GPU and have a
  *          long K run tiles of up to 256 pixels, one CTA per SM, or two SMs per tile.
+ *          "norm_form" (0 = default: by size, 1 .. 5; read by the next load_module): group_norm as rows by warps, rows by blocks, slab, streamed
+ *          or strided, where a tensor can (tpucb_interp_get_op_form says what was taken).
+ *          "linear_tiles" (1 = default: by size, 1000 * CTAs that share a tile's K (1 .. 8) + channels per tile (16 .. 256, a multiple of 16;
+ *          FP32: rows, 8 .. 56, of 8), 10000 + channels (64, 128, 192, 256): two SMs per tile, BF16 only; read by the next load_module):
+ *          how inner products with activation or residual run.
  *          "fuse_activations" (0/1, default 1; read by the next load_module): run each
  *          quant(INT8->BF16) -> slope-table activation -> quant(BF16->INT8) chain as one launch
  *          that still writes all three tensors.
@@ -160,7 +179,7 @@ int tpucb_interp_get_op_form(tpucb_interp *it, const char *name, char *out, size
  *          self-test of the error path. Every wait inside the tensor-core kernels is bounded (1024 rounds of 1024
  *          polls); when one runs out the kernel records a code in the interpreter's device error word, drains its
  *          copies, frees its tensor memory and returns, and the next tpucb_interp_sync / invoke reports it as an
- *          error status while the interpreter stays usable. With this option the tensor-core convolutions of the next
+ *          error status while the interpreter stays usable. With this option the tensor-core kernels of the next
  *          module never hand their accumulator back and wait only `rounds` rounds, so that exactly this happens.
  *          "fuse_residual_add" (0 never, 1 always, 2 = default: by size; read by the next load_module; needs fuse_activations): an INT8
  *          two-input eltwise add (or a BF16 one with ReLU) whose later-produced operand is a tensor-core convolution that feeds nothing else
