@@ -191,12 +191,12 @@ int norm(int n, int pixels, int c, int groups, int es, int sms, int mode) {
   } else if (p.form == NORM_SLAB || p.form == NORM_STREAMED) {
     const bool slab = p.form == NORM_SLAB;
     EXPECT(p.threads == (slab ? kSlabThreads : kStreamThreads));
-    EXPECT(p.chunks <= 65535 && p.chunk_groups >= 1 && p.chunk_groups <= 256 && (long long)p.chunks * p.chunk_groups >= groups);
+    EXPECT(p.chunk_groups >= 1 && p.chunk_groups <= 256 && (long long)p.chunks * p.chunk_groups >= groups);
     EXPECT((p.chunks - 1) * p.chunk_groups < groups);
     EXPECT((long long)p.vecs * N >= (long long)p.chunk_groups * cg && (p.chunks == 1 || p.chunk_groups * cg == p.vecs * N));
     EXPECT(p.lanes >= 1 && p.vecs * p.lanes <= (int)p.threads && p.nv * p.lanes >= p.part_pixels && p.col_split >= 1);
     EXPECT((long long)p.parts * p.part_pixels >= pixels && (long long)(p.parts - 1) * p.part_pixels < pixels);
-    EXPECT(p.grid == (unsigned)(n * p.parts) && p.part_pixels <= 1 << 22);
+    EXPECT(p.grid == (unsigned)(n * p.chunks * p.parts) && (long long)n * p.chunks * p.parts < 1LL << 31 && p.part_pixels <= 1 << 22);
     const int per = p.aligned ? 1 : N, group_width = p.aligned ? cg / N : cg;
     EXPECT(p.group_span % 32 == 0 && p.group_span >= p.col_split * group_width);
     const size_t tab = ((size_t)p.threads * per + (size_t)p.chunk_groups * (p.group_span + p.group_span / 32)) * 4;
@@ -206,7 +206,7 @@ int norm(int n, int pixels, int c, int groups, int es, int sms, int mode) {
     } else {
       EXPECT(p.smem <= 48 * 1024 && p.smem >= tab + (size_t)p.chunk_groups * 4 && p.smem >= (size_t)p.chunk_groups * 8);
       EXPECT((long long)p.apply_parts * p.apply_pixels >= pixels && (long long)(p.apply_parts - 1) * p.apply_pixels < pixels);
-      EXPECT(p.apply_grid == (unsigned)(n * p.apply_parts) && p.apply_pixels <= 1 << 22);
+      EXPECT(p.apply_grid == (unsigned)(n * p.chunks * p.apply_parts) && p.apply_pixels <= 1 << 22);
     }
   } else {
     EXPECT(p.parts <= (int)p.threads && p.grid == (unsigned)(n * groups * p.parts) && (long long)n * groups * p.parts < 1LL << 31);

@@ -256,9 +256,10 @@ template <typename T, int THREADS> struct NormTile { // (parts: of the image, of
   int v, p, lanes, ch;                         // the thread's vector column, pixel lane, pixel lanes of the block, first channel
   bool active;
   __device__ __forceinline__ NormTile(const GroupNormArgs &a, unsigned block, int parts, int pixels) {
-    img = parts == 1 ? block : block / parts;
-    part = block - img * parts;
-    chunk = blockIdx.y;
+    const int slab = parts == 1 ? block : block / parts;
+    part = block - slab * parts;
+    img = a.chunks == 1 ? slab : slab / a.chunks;
+    chunk = slab - img * a.chunks; // (chunks of a pixel that share a line of the L2 are neighbours in the grid)
     first_group = chunk * a.chunk_groups;
     n_groups = min(a.chunk_groups, a.groups - first_group);
     px0 = part * pixels;
@@ -685,15 +686,15 @@ inline void launch_group_norm(const GroupNormArgs &a, const GroupNormPlan &p, bo
       break;
     case NORM_ROWS_BLOCK: by_nv([&](auto nv) { by_rows(nv, std::integral_constant<int, 0>()); }); break;
     case NORM_SLAB:
-      if (p.aligned) launch_cluster_k(a.parts, group_norm_slab_kernel<T, true>, dim3(p.grid, a.chunks), p.threads, p.smem, s, a);
-      else launch_cluster_k(a.parts, group_norm_slab_kernel<T, false>, dim3(p.grid, a.chunks), p.threads, p.smem, s, a);
+      if (p.aligned) launch_cluster_k(a.parts, group_norm_slab_kernel<T, true>, p.grid, p.threads, p.smem, s, a);
+      else launch_cluster_k(a.parts, group_norm_slab_kernel<T, false>, p.grid, p.threads, p.smem, s, a);
       break;
     case NORM_STREAMED: {
       auto both_passes = [&](auto aligned) {
         constexpr bool A = decltype(aligned)::value;
-        launch_k(group_norm_stats_kernel<T, A>, dim3(p.grid, a.chunks), p.threads, p.smem, s, a);
+        launch_k(group_norm_stats_kernel<T, A>, p.grid, p.threads, p.smem, s, a);
         PdlConvScope overlap; // the second pass fetches gamma and beta while the first ends
-        launch_k(group_norm_apply_kernel<T, A>, dim3(p.apply_grid, a.chunks), p.threads, (size_t)a.chunk_groups * sizeof(float2), s, a);
+        launch_k(group_norm_apply_kernel<T, A>, p.apply_grid, p.threads, (size_t)a.chunk_groups * sizeof(float2), s, a);
       };
       if (p.aligned) both_passes(std::true_type());
       else both_passes(std::false_type());

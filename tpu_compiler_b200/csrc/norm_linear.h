@@ -155,7 +155,7 @@ inline GroupNormPlan group_norm_plan(int n, int pixels, int c, int groups, int e
     }
   }
   // chunks: whole groups and whole vectors; the smallest such unit, or the whole row
-  if (c >= 1 << 19 || (long long)n * 8 >= 1LL << 31) return strided; // (small_div; the grid, 65535 chunks)
+  if (c >= 1 << 19 || lots * 8 >= 1LL << 31) return strided; // (small_div; the grid)
   int unit_groups = 1;
   while (unit_groups < groups && unit_groups * cg % N) ++unit_groups;
   const int unit_vecs = (unit_groups * cg + N - 1) / N;
@@ -172,19 +172,26 @@ inline GroupNormPlan group_norm_plan(int n, int pixels, int c, int groups, int e
     p.lanes = threads / p.vecs;
     p.nv = (p.part_pixels + p.lanes - 1) / p.lanes;
     p.threads = (unsigned)threads;
-    p.grid = (unsigned)((long long)n * p.parts); // x chunks
+    p.grid = (unsigned)((long long)n * p.chunks * p.parts);
     // a column's pixel lanes are summed by several threads where there are few columns, eight lanes or more each
     const int group_width = p.aligned ? cg / N : cg;
     p.col_split = std::max(1, std::min(threads / (p.vecs * per), p.lanes / 8));
     p.group_span = round_up(p.col_split * group_width, 32);
     p.smem = ((size_t)threads * per + (size_t)p.chunk_groups * p.group_span / 32 * 33 + round_up(p.chunk_groups, 2)) * 4;
   };
-  // slab: 64 bytes of a pixel and more, in the shared memory of at most eight blocks. Few blocks are best, for the sums of each cost the same: at
-  // most six where fewer hold it (2 x 320 x 96 x 96 us with three modules in flight / alone: by four 7.7 / 18.5, six 9.0 / 16.4, eight 11.3 /
-  // 22.6, streamed 11.6 / 22.6). Where a block leaves no room for a second one on its SM, nothing fills the time of its loads and sums: then only if
-  // they run at once and on half of the SMs, else by more blocks (16 x 256 x 64 x 64 by two 17.8 / 22.6, by three 16.3 / 22.3, streamed 18.8 / 28.5;
-  // 6 x 62 x 100 x 100 by seven 6.2 / 16.4, streamed 6.1 / 12.3).
-  const int wide = (4 + unit_vecs - 1) / unit_vecs;
+  // Tensors whose passes take long enough that only their loops count: from 128 vectors per thread of the streamed form on.
+  const bool large = (long long)n * pixels * ((c + N - 1) / N) >= 128LL * kStreamThreads * sm_count;
+  // slab: 64 bytes of a pixel and more, in the shared memory of at most eight blocks; more of a pixel while two blocks per SM remain and one
+  // block holds it (40 x 1280 x 16 x 16 by 80 bytes 24.9 us with three modules in flight / 28.7 alone, by 320 10.6 / 18.5, streamed 19.1 / 32.8). Few blocks
+  // per slab are best, for the sums of each cost the same: at most six where fewer hold it (2 x 320 x 96 x 96: by four 7.7 / 18.5, six 9.0 / 16.4,
+  // eight 11.3 / 22.6, streamed 11.6 / 22.6). Where a block leaves no room for a second one on its SM, nothing fills the time of its loads and sums:
+  // then only if they run at once and on half of the SMs, else by more blocks (16 x 256 x 64 x 64 by two 17.8 / 22.6, by three 16.3 / 22.3,
+  // streamed 18.8 / 28.5; 6 x 62 x 100 x 100 by seven 6.2 / 16.4, streamed 6.1 / 12.3). Large tensors only without clusters (100 x 640 x 32 x 32
+  // 70.5 / 80, streamed 77.8 / 115; by clusters of four 48 x 320 x 64 x 64 82 / 92, streamed 72.6 / 94).
+  int wide = (4 + unit_vecs - 1) / unit_vecs;
+  while (2 * wide * unit_vecs <= kSlabThreads && (long long)n * ((units + 2 * wide - 1) / (2 * wide)) >= 2LL * sm_count &&
+         (long long)pixels * 2 * wide * unit_vecs * 16 <= 90 * 1024)
+    wide *= 2;
   lay_out(kSlabThreads, wide, 1);
   if (mode != 1 + NORM_STREAMED) {
     const size_t fixed = p.smem + (size_t)p.chunk_groups * 16, half = 113 * 1024;
@@ -194,7 +201,7 @@ inline GroupNormPlan group_norm_plan(int n, int pixels, int c, int groups, int e
       return held ? (int)std::min(9LL, (pixels + held * lanes - 1) / (held * lanes)) : 9;
     };
     auto try_slab = [&](int parts) {
-      if (parts > 8) return false;
+      if (parts > 8 || (large && parts > 1 && mode == 0)) return false;
       lay_out(kSlabThreads, wide, parts);
       p.smem = fixed + (size_t)p.nv * kSlabThreads * 16;
       p.form = NORM_SLAB;
@@ -213,14 +220,12 @@ inline GroupNormPlan group_norm_plan(int n, int pixels, int c, int groups, int e
   // Blocks per SM of the two passes. Few leave fewer partial statistics and less around the loops, many hide the memory's latency; us alone /
   // with three modules in flight, (1, 1), (1, 2), (2, 3): 4 x 128 x 128 x 128 24.6 / 10.7, 22.5 / 12.0, 20.5 / 13.8; 8 x 320 x 64 x 64
   // 28.7 / 14.1, 26.6 / 15.2, 22.6 / 16.5; 1 x 256 x 512 x 512 106 / 65, 91 / 71, 85 / 66; fp32 2 x 100 x 400 x 400 129 / 83, 116 / 83, 90 / 70.
-  // From 128 vectors per thread on the loops are all that counts.
-  const bool large = slabs * pixels * p.vecs >= 128LL * kStreamThreads * sm_count;
   const int fs = large ? 2 : 1, fa = large ? 3 : 2;
   const int apply = parts_of(fa);
   lay_out(kStreamThreads, most_units, std::max(parts_of(fs), (int)((pixels + (1LL << 22) - 1) >> 22))); // (small_div)
   p.apply_pixels = (pixels + std::max(apply, p.parts) - 1) / std::max(apply, p.parts);
   p.apply_parts = (pixels + p.apply_pixels - 1) / p.apply_pixels;
-  p.apply_grid = (unsigned)((long long)n * p.apply_parts);
+  p.apply_grid = (unsigned)((long long)n * p.chunks * p.apply_parts);
   p.form = NORM_STREAMED;
   return p;
 }
