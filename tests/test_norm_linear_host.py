@@ -190,7 +190,7 @@ int norm(int n, int pixels, int c, int groups, int es, int sms, int mode) {
     EXPECT(p.threads % 32 == 0 && p.threads <= 512 && (p.rows == 1 || p.nv <= 4));
   } else if (p.form == NORM_SLAB || p.form == NORM_STREAMED) {
     const bool slab = p.form == NORM_SLAB;
-    EXPECT(p.threads == (slab ? kSlabThreads : kStreamThreads));
+    EXPECT(slab ? p.threads == kSlabThreads || (p.threads == kSmallSlabThreads && p.parts == 1 && p.smem <= 48 * 1024) : p.threads == kStreamThreads);
     EXPECT(p.chunk_groups >= 1 && p.chunk_groups <= 256 && (long long)p.chunks * p.chunk_groups >= groups);
     EXPECT((p.chunks - 1) * p.chunk_groups < groups);
     EXPECT((long long)p.vecs * N >= (long long)p.chunk_groups * cg && (p.chunks == 1 || p.chunk_groups * cg == p.vecs * N));
@@ -202,7 +202,7 @@ int norm(int n, int pixels, int c, int groups, int es, int sms, int mode) {
     const size_t tab = ((size_t)p.threads * per + (size_t)p.chunk_groups * (p.group_span + p.group_span / 32)) * 4;
     if (slab) {
       EXPECT(p.parts <= 8 && p.smem <= 227 * 1024);
-      EXPECT(p.smem >= tab + (size_t)p.nv * kSlabThreads * 16 + (size_t)p.chunk_groups * 16);
+      EXPECT(p.smem >= tab + (size_t)p.nv * p.threads * 16 + (size_t)p.chunk_groups * 16);
     } else {
       EXPECT(p.smem <= 48 * 1024 && p.smem >= tab + (size_t)p.chunk_groups * 4 && p.smem >= (size_t)p.chunk_groups * 8);
       EXPECT((long long)p.apply_parts * p.apply_pixels >= pixels && (long long)(p.apply_parts - 1) * p.apply_pixels < pixels);

@@ -340,58 +340,53 @@ __device__ __forceinline__ void own_means(const GroupNormArgs &a, int ch, int fi
     for (int j = 0; j < NormVec<T>::P; ++j) m[j] = Pair(v[2 * j], v[2 * j + 1]);
   }
 }
-// What a thread sums: distances from its first value and their squares, per channel or, where vectors lie within groups, in all.
-template <typename T, bool ALIGNED> struct NormMoments {
-  typedef NormVec<T> V;
-  static constexpr int P = ALIGNED ? 1 : V::P;
-  Pair first[P] = {}, s[P] = {}, q[P] = {}; // first: negative
-  __device__ __forceinline__ void begin(const uint4 &raw) {
-    Pair x[V::P];
-    V::get(raw, x);
+// What a thread of a slab sums: distances from its first value and their squares, per channel or, where vectors lie within groups, in all.
+template <typename T, bool ALIGNED> constexpr int kMoments = ALIGNED ? 1 : NormVec<T>::P;
+template <typename T, bool ALIGNED> __device__ __forceinline__ void moments_take(const uint4 &raw, const Pair *first, Pair *s, Pair *q) { // first: negative
+  Pair x[NormVec<T>::P];
+  NormVec<T>::get(raw, x);
 #pragma unroll
-    for (int j = 0; j < P; ++j) {
-      first[j] = ALIGNED ? both(-x[0].lo()) : x[j] * both(-1.0f);
-      s[j] = q[j] = both(0.0f);
-    }
+  for (int j = 0; j < NormVec<T>::P; ++j) {
+    const int i = ALIGNED ? 0 : j;
+    const Pair d = x[j] + first[i];
+    s[i] = s[i] + d;
+    q[i] = fma(d, d, q[i]);
   }
-  __device__ __forceinline__ void take(const uint4 &raw) {
-    Pair x[V::P];
-    V::get(raw, x);
+}
+template <typename T, bool ALIGNED> __device__ __forceinline__ void moments_begin(const uint4 &raw, Pair *first) {
+  Pair x[NormVec<T>::P];
+  NormVec<T>::get(raw, x);
 #pragma unroll
-    for (int j = 0; j < V::P; ++j) {
-      const int i = ALIGNED ? 0 : j;
-      const Pair d = x[j] + first[i];
-      s[i] = s[i] + d;
-      q[i] = fma(d, d, q[i]);
-    }
+  for (int j = 0; j < kMoments<T, ALIGNED>; ++j) first[j] = ALIGNED ? both(-x[0].lo()) : x[j] * both(-1.0f);
+}
+// The block's mean and M2 of each group of its chunk, from `mine` vectors of each thread: `done(group of the chunk, mean, M2)` in one thread
+// each. mean_of: [groups of the chunk]; tab: norm_group_sums. (Where vectors lie within groups both halves of the pairs count as columns.)
+template <typename T, bool ALIGNED, int THREADS, class Done>
+__device__ __forceinline__ void moments_join(const GroupNormArgs &a, const NormTile<T, THREADS> &t, int mine, Pair *first, const Pair *s, Pair *q, float *mean_of,
+                                             float *tab, Done done) {
+  constexpr int P = kMoments<T, ALIGNED>;
+  const float n = (float)mine * (ALIGNED ? NormVec<T>::P : 1), inv = mine > 0 ? 1.0f / n : 0.0f;
+  const float inv_count = 1.0f / ((float)(t.px1 - t.px0) * (float)a.cg);
+  Pair x[P];
+#pragma unroll
+  for (int j = 0; j < P; ++j) {
+    const Pair mean = s[j] * both(inv);
+    q[j] = fma(s[j] * both(-1.0f), mean, q[j]);
+    q[j] = Pair(q[j].lo() < 0.0f ? 0.0f : q[j].lo(), q[j].hi() < 0.0f ? 0.0f : q[j].hi()); // (a NaN stays)
+    first[j] = fma(first[j], both(-1.0f), mean); // the mean
+    x[j] = first[j] * both(n);
   }
-  // The block's mean and M2 of each group of its chunk, from `mine` vectors of each thread: `done(group of the chunk, mean, M2)` in one thread
-  // each. mean_of: [groups of the chunk]; tab: norm_group_sums. (Where vectors lie within groups both halves of the pairs count as columns.)
-  template <int THREADS, class Done>
-  __device__ __forceinline__ void join(const GroupNormArgs &a, const NormTile<T, THREADS> &t, int mine, float *mean_of, float *tab, Done done) {
-    const float n = (float)mine * (ALIGNED ? V::P : 1), inv = mine > 0 ? 1.0f / n : 0.0f;
-    const float inv_count = 1.0f / ((float)(t.px1 - t.px0) * (float)a.cg);
-    Pair x[P];
+  norm_group_sums<T, ALIGNED, THREADS>(a, t, x, tab, [&](int g, float sum) { mean_of[g] = sum * inv_count; });
+  __syncthreads();
+  Pair m[P];
+  own_means<T, ALIGNED>(a, t.ch, t.first_group, t.n_groups, [&](int g) { return mean_of[g]; }, m);
 #pragma unroll
-    for (int j = 0; j < P; ++j) {
-      const Pair mean = s[j] * both(inv);
-      q[j] = fma(s[j] * both(-1.0f), mean, q[j]);
-      q[j] = Pair(q[j].lo() < 0.0f ? 0.0f : q[j].lo(), q[j].hi() < 0.0f ? 0.0f : q[j].hi()); // (a NaN stays)
-      first[j] = fma(first[j], both(-1.0f), mean); // the mean
-      x[j] = mine > 0 ? first[j] * both(n) : both(0.0f);
-    }
-    norm_group_sums<T, ALIGNED, THREADS>(a, t, x, tab, [&](int g, float sum) { mean_of[g] = sum * inv_count; });
-    __syncthreads();
-    Pair m[P];
-    own_means<T, ALIGNED>(a, t.ch, t.first_group, t.n_groups, [&](int g) { return mean_of[g]; }, m);
-#pragma unroll
-    for (int j = 0; j < P; ++j) {
-      const Pair d = first[j] + m[j];
-      x[j] = mine > 0 ? fma(d * both(n), d, q[j]) : both(0.0f);
-    }
-    norm_group_sums<T, ALIGNED, THREADS>(a, t, x, tab, [&](int g, float sum) { done(g, mean_of[g], sum); });
+  for (int j = 0; j < P; ++j) {
+    const Pair d = first[j] + m[j];
+    x[j] = mine > 0 ? fma(d * both(n), d, q[j]) : both(0.0f);
   }
-};
+  norm_group_sums<T, ALIGNED, THREADS>(a, t, x, tab, [&](int g, float sum) { done(g, mean_of[g], sum); });
+}
 // y = x scale + shift of a thread's channels
 template <typename T> struct NormAffine {
   typedef NormVec<T> V;
@@ -435,38 +430,43 @@ template <typename T> struct NormAffine {
 // there are any: 64 x 256 x 32 x 32 with SiLU 14.2 us with three modules in flight (72% of the memory's rate), 8 x 320 x 64 x 64 12.8, alone
 // 18.5. (With the vectors in registers, eight per thread, those took 22.8, 25.1 and 28.7 us: a wave of blocks held half as much, in one block
 // per SM.)
-template <typename T, bool ALIGNED> __global__ void __launch_bounds__(kSlabThreads, 2) group_norm_slab_kernel(const GroupNormArgs a) {
+template <typename T, bool ALIGNED, int THREADS> __global__ void __launch_bounds__(THREADS, 1024 / THREADS) group_norm_slab_kernel(const GroupNormArgs a) {
   extern __shared__ __align__(16) float smem[];
   uint4 *held = reinterpret_cast<uint4 *>(smem) + threadIdx.x;
-  float2 *own = reinterpret_cast<float2 *>(smem + (size_t)a.held * kSlabThreads * 4); // [groups of the chunk]: this block's mean and M2
+  float2 *own = reinterpret_cast<float2 *>(smem + (size_t)a.held * THREADS * 4); // [groups of the chunk]: this block's mean and M2
   float2 *all = own + a.chunk_groups;                                                 // mean and 1 / sqrt(var + eps) of the image
   float *tab = reinterpret_cast<float *>(all + a.chunk_groups);
-  const NormTile<T, kSlabThreads> t(a, blockIdx.x, a.parts, a.part_pixels);
+  const NormTile<T, THREADS> t(a, blockIdx.x, a.parts, a.part_pixels);
   const size_t at = t.offset(a, t.px0 + t.p), step = (size_t)t.lanes * a.cp;
   const int mine = t.active && t.px0 + t.p < t.px1 ? small_div(t.px1 - t.px0 - t.p + t.lanes - 1, a.inv_lanes) : 0;
-  norm_clear<T, ALIGNED, kSlabThreads>(a, tab);
+  norm_clear<T, ALIGNED, THREADS>(a, tab);
   pdl_prologue();
   {
     const T *in = (const T *)a.in + at;
     uint32_t to = ptx::smem_u32(held);
 #pragma unroll 4
-    for (int k = 0; k < mine; ++k, in += step, to += kSlabThreads * 16)
+    for (int k = 0; k < mine; ++k, in += step, to += THREADS * 16)
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(in) : "memory");
     asm volatile("cp.async.wait_all;" ::: "memory");
   }
-  NormMoments<T, ALIGNED> moments;
-  moments.begin(mine > 0 ? held[0] : make_uint4(0u, 0u, 0u, 0u));
+  constexpr int P = kMoments<T, ALIGNED>;
+  Pair first[P], sum[P], square[P];
+#pragma unroll
+  for (int j = 0; j < P; ++j) first[j] = sum[j] = square[j] = both(0.0f);
+  if (mine > 0) {
+    moments_begin<T, ALIGNED>(held[0], first);
 #pragma unroll 4
-  for (int k = 0; k < mine; ++k) moments.take(held[k * kSlabThreads]);
+    for (int k = 0; k < mine; ++k) moments_take<T, ALIGNED>(held[k * THREADS], first, sum, square);
+  }
   float *mean_of = reinterpret_cast<float *>(all);
-  moments.template join<kSlabThreads>(a, t, mine, mean_of, tab, [&](int g, float mean, float m2) { own[g] = make_float2(mean, m2); });
+  moments_join<T, ALIGNED>(a, t, mine, first, sum, square, mean_of, tab, [&](int g, float mean, float m2) { own[g] = make_float2(mean, m2); });
   NormAffine<T> affine;
   if (t.active) affine.load(a, t.ch);
   if (a.parts > 1) ptx::cluster_sync();
   else __syncthreads();
   const float total = (float)a.pixels * (float)a.cg;
   if (a.parts == 1) {
-    for (int g = threadIdx.x; g < t.n_groups; g += kSlabThreads) all[g] = make_float2(own[g].x, rsqrtf(own[g].y / total + a.eps));
+    for (int g = threadIdx.x; g < t.n_groups; g += THREADS) all[g] = make_float2(own[g].x, rsqrtf(own[g].y / total + a.eps));
   } else {
     // eight threads per group, one block's numbers each (a thread that read them all took a round trip for each: 2 x 320 x 96 x 96 by 8
     // blocks 12.7 us with three modules in flight instead of 11.3)
@@ -477,7 +477,7 @@ template <typename T, bool ALIGNED> __global__ void __launch_bounds__(kSlabThrea
       for (int k = 4; k; k /= 2) v += __shfl_xor_sync(0xffffffffu, v, k);
       return v;
     };
-    for (int first = 0; first < t.n_groups; first += kSlabThreads / 8) {
+    for (int first = 0; first < t.n_groups; first += THREADS / 8) {
       const int g = min(first + (int)threadIdx.x / 8, t.n_groups - 1);
       float2 o = make_float2(0.0f, 0.0f);
       if (r < a.parts)
@@ -496,7 +496,7 @@ template <typename T, bool ALIGNED> __global__ void __launch_bounds__(kSlabThrea
     with_activation(a.act, [&](auto act) {
 #pragma unroll 2
       for (int k = 0; k < mine; ++k)
-        *reinterpret_cast<uint4 *>(out + at + k * step) = affine.template apply<decltype(act)::value>(held[k * kSlabThreads], valid);
+        *reinterpret_cast<uint4 *>(out + at + k * step) = affine.template apply<decltype(act)::value>(held[k * THREADS], valid);
     });
   }
   __syncwarp();
@@ -504,10 +504,9 @@ template <typename T, bool ALIGNED> __global__ void __launch_bounds__(kSlabThrea
 }
 
 // ---- streamed
-// begin(the first vector) and use(vector, index) for `count` vectors that are `step` values apart, the next D of them on their way while D are used (with one set of
+// use(vector, index) for `count` vectors that are `step` values apart, the next D of them on their way while D are used (with one set of
 // four and no way ahead: 4 x 128 x 128 x 128 12.3 us with three modules in flight instead of 10.7, fp32 2 x 100 x 400 x 400 165 instead of 70).
-template <int D, typename T, class Begin, class Use>
-__device__ __forceinline__ void for_vectors(const T *p, long long step, int count, Begin begin, Use use) {
+template <int D, typename T, class Use> __device__ __forceinline__ void for_vectors(const T *p, long long step, int count, Use use) {
   uint4 r[2][D];
   auto fetch = [&](uint4 (&to)[D], int k) {
 #pragma unroll
@@ -520,7 +519,6 @@ __device__ __forceinline__ void for_vectors(const T *p, long long step, int coun
       if (k + i < count) use(from[i], k + i);
   };
   fetch(r[0], 0);
-  begin(r[0][0]);
   for (int k = 0; k < count; k += 2 * D) {
     fetch(r[1], k + D);
     each(r[0], k);
@@ -529,6 +527,8 @@ __device__ __forceinline__ void for_vectors(const T *p, long long step, int coun
   }
 }
 
+// The slab's sums, written out: through moments_join the compiled loop is slower where groups are no whole vectors (6 x 320 x 128 x 128 46.4 us with
+// three modules in flight instead of 38.9; the registers are the same).
 template <typename T, bool ALIGNED> __global__ void __launch_bounds__(kStreamThreads, 3) group_norm_stats_kernel(const GroupNormArgs a) {
   extern __shared__ float smem[];
   const NormTile<T, kStreamThreads> t(a, blockIdx.x, a.parts, a.part_pixels);
@@ -537,12 +537,56 @@ template <typename T, bool ALIGNED> __global__ void __launch_bounds__(kStreamThr
   norm_clear<T, ALIGNED, kStreamThreads>(a, tab);
   pdl_prologue();
   const int mine = t.active && t.px0 + t.p < t.px1 ? small_div(t.px1 - t.px0 - t.p + t.lanes - 1, a.inv_lanes) : 0;
-  const T *in = (const T *)a.in + (mine > 0 ? t.offset(a, t.px0 + t.p) : 0);
-  NormMoments<T, ALIGNED> moments;
-  if (mine > 0) for_vectors<ALIGNED ? 4 : 2>(in, (long long)t.lanes * a.cp, mine, [&](const uint4 &raw) { moments.begin(raw); }, [&](const uint4 &raw, int) { moments.take(raw); });
+  typedef NormVec<T> V;
+  constexpr int P = ALIGNED ? 1 : V::P;
+  Pair first[P], s[P], q[P]; // first: negative
+#pragma unroll
+  for (int j = 0; j < P; ++j) first[j] = s[j] = q[j] = both(0.0f);
+  auto take = [&](const uint4 &raw) {
+    Pair x[V::P];
+    V::get(raw, x);
+#pragma unroll
+    for (int j = 0; j < V::P; ++j) {
+      const int i = ALIGNED ? 0 : j;
+      const Pair d = x[j] + first[i];
+      s[i] = s[i] + d;
+      q[i] = fma(d, d, q[i]);
+    }
+  };
+  if (mine > 0) {
+    const T *at = (const T *)a.in + t.offset(a, t.px0 + t.p);
+    const size_t step = (size_t)t.lanes * a.cp;
+    {
+      Pair x[V::P];
+      V::get(*reinterpret_cast<const uint4 *>(at), x);
+#pragma unroll
+      for (int j = 0; j < P; ++j) first[j] = ALIGNED ? both(-x[0].lo()) : x[j] * both(-1.0f);
+    }
+    for_vectors<ALIGNED ? 4 : 2>(at, (long long)step, mine, [&](const uint4 &raw, int) { take(raw); });
+  }
+  // The thread's count, mean and M2 (per channel; where vectors lie within groups both halves count as columns of their own)
+  const float n = (float)mine * (ALIGNED ? V::P : 1), inv = mine > 0 ? 1.0f / n : 0.0f;
+  const float inv_count = 1.0f / ((float)(t.px1 - t.px0) * (float)a.cg);
+  Pair x[P];
+#pragma unroll
+  for (int j = 0; j < P; ++j) {
+    const Pair mean = s[j] * both(inv);
+    q[j] = fma(s[j] * both(-1.0f), mean, q[j]);
+    q[j] = Pair(q[j].lo() < 0.0f ? 0.0f : q[j].lo(), q[j].hi() < 0.0f ? 0.0f : q[j].hi()); // (a NaN stays)
+    first[j] = fma(first[j], both(-1.0f), mean); // the mean
+    x[j] = first[j] * both(n);
+  }
+  norm_group_sums<T, ALIGNED, kStreamThreads>(a, t, x, tab, [&](int g, float sum) { mean_of[g] = sum * inv_count; });
+  __syncthreads();
+  Pair m[P];
+  own_means<T, ALIGNED>(a, t.ch, t.first_group, t.n_groups, [&](int g) { return mean_of[g]; }, m);
+#pragma unroll
+  for (int j = 0; j < P; ++j) {
+    const Pair d = first[j] + m[j];
+    x[j] = mine > 0 ? fma(d * both(n), d, q[j]) : both(0.0f);
+  }
   float2 *partial = a.partial + ((size_t)t.img * a.groups + t.first_group) * a.parts;
-  moments.template join<kStreamThreads>(a, t, mine, mean_of, tab,
-                                        [&](int g, float mean, float m2) { partial[(size_t)g * a.parts + t.part] = make_float2(mean, m2); });
+  norm_group_sums<T, ALIGNED, kStreamThreads>(a, t, x, tab, [&](int g, float sum) { partial[(size_t)g * a.parts + t.part] = make_float2(mean_of[g], sum); });
 }
 
 template <typename T, bool ALIGNED> __global__ void __launch_bounds__(kStreamThreads, 3) group_norm_apply_kernel(const GroupNormArgs a) {
@@ -579,7 +623,7 @@ template <typename T, bool ALIGNED> __global__ void __launch_bounds__(kStreamThr
   const size_t at = t.offset(a, t.px0 + t.p) + (size_t)max(mine - 1, 0) * step;
   T *out = (T *)a.out + at;
   with_activation(a.act, [&](auto act) {
-    for_vectors<4>((const T *)a.in + at, -(long long)step, mine, [](const uint4 &) {}, [&](const uint4 &raw, int k) {
+    for_vectors<4>((const T *)a.in + at, -(long long)step, mine, [&](const uint4 &raw, int k) {
       *reinterpret_cast<uint4 *>(out - k * step) = affine.template apply<decltype(act)::value>(raw, valid);
     });
   });
@@ -647,17 +691,17 @@ template <typename T> __global__ void group_norm_strided_apply_kernel(const Grou
 
 // To be called at load, on the device that will run it (conv_kernel_ready).
 inline void group_norm_ready(const GroupNormPlan &p, bool f32) {
-  if (p.form != NORM_SLAB) return;
+  if (p.form != NORM_SLAB || p.threads != kSlabThreads) return; // (small slabs stay below what a kernel has unasked)
   int device = 0;
   TPUCB_CUDA(cudaGetDevice(&device));
   auto set = [&](auto k) {
     static OncePerDevice ready; // one of each kernel
     ready.run(device, [] { TPUCB_CUDA(cudaFuncSetAttribute(decltype(k)::value, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024)); });
   };
-  if (f32 && p.aligned) set(KernelConstant<group_norm_slab_kernel<float, true>>());
-  else if (f32) set(KernelConstant<group_norm_slab_kernel<float, false>>());
-  else if (p.aligned) set(KernelConstant<group_norm_slab_kernel<uint16_t, true>>());
-  else set(KernelConstant<group_norm_slab_kernel<uint16_t, false>>());
+  if (f32 && p.aligned) set(KernelConstant<group_norm_slab_kernel<float, true, kSlabThreads>>());
+  else if (f32) set(KernelConstant<group_norm_slab_kernel<float, false, kSlabThreads>>());
+  else if (p.aligned) set(KernelConstant<group_norm_slab_kernel<uint16_t, true, kSlabThreads>>());
+  else set(KernelConstant<group_norm_slab_kernel<uint16_t, false, kSlabThreads>>());
 }
 inline void launch_group_norm(const GroupNormArgs &a, const GroupNormPlan &p, bool f32, cudaStream_t s) {
   auto by_type = [&](auto type) {
@@ -686,8 +730,13 @@ inline void launch_group_norm(const GroupNormArgs &a, const GroupNormPlan &p, bo
       break;
     case NORM_ROWS_BLOCK: by_nv([&](auto nv) { by_rows(nv, std::integral_constant<int, 0>()); }); break;
     case NORM_SLAB:
-      if (p.aligned) launch_cluster_k(a.parts, group_norm_slab_kernel<T, true>, p.grid, p.threads, p.smem, s, a);
-      else launch_cluster_k(a.parts, group_norm_slab_kernel<T, false>, p.grid, p.threads, p.smem, s, a);
+      if (p.threads == kSlabThreads) {
+        if (p.aligned) launch_cluster_k(a.parts, group_norm_slab_kernel<T, true, kSlabThreads>, p.grid, p.threads, p.smem, s, a);
+        else launch_cluster_k(a.parts, group_norm_slab_kernel<T, false, kSlabThreads>, p.grid, p.threads, p.smem, s, a);
+      } else {
+        if (p.aligned) launch_k(group_norm_slab_kernel<T, true, kSmallSlabThreads>, p.grid, p.threads, p.smem, s, a);
+        else launch_k(group_norm_slab_kernel<T, false, kSmallSlabThreads>, p.grid, p.threads, p.smem, s, a);
+      }
       break;
     case NORM_STREAMED: {
       auto both_passes = [&](auto aligned) {

@@ -99,7 +99,7 @@ inline LinearSpec linear_spec(const ParsedOp &op, const DevTensor &in, const Dev
 
 // ---- how a group norm runs (group_norm.cuh)
 enum NormForm { NORM_ROWS_WARP = 0, NORM_ROWS_BLOCK, NORM_SLAB, NORM_STREAMED, NORM_STRIDED };
-constexpr int kSlabThreads = 512, kStreamThreads = 256;
+constexpr int kSlabThreads = 512, kSmallSlabThreads = 128, kStreamThreads = 256;
 struct GroupNormPlan {
   int form = NORM_STRIDED;
   unsigned grid = 0, threads = 256;
@@ -182,12 +182,14 @@ inline GroupNormPlan group_norm_plan(int n, int pixels, int c, int groups, int e
   // Tensors whose passes take long enough that only their loops count: from 128 vectors per thread of the streamed form on.
   const bool large = (long long)n * pixels * ((c + N - 1) / N) >= 128LL * kStreamThreads * sm_count;
   // slab: 64 bytes of a pixel and more, in the shared memory of at most eight blocks; more of a pixel while two blocks per SM remain and one
-  // block holds it (40 x 1280 x 16 x 16 by 80 bytes 24.9 us with three modules in flight / 28.7 alone, by 320 10.6 / 18.5, streamed 19.1 / 32.8). Few blocks
-  // per slab are best, for the sums of each cost the same: at most six where fewer hold it (2 x 320 x 96 x 96: by four 7.7 / 18.5, six 9.0 / 16.4,
-  // eight 11.3 / 22.6, streamed 11.6 / 22.6). Where a block leaves no room for a second one on its SM, nothing fills the time of its loads and sums:
-  // then only if they run at once and on half of the SMs, else by more blocks (16 x 256 x 64 x 64 by two 17.8 / 22.6, by three 16.3 / 22.3,
-  // streamed 18.8 / 28.5; 6 x 62 x 100 x 100 by seven 6.2 / 16.4, streamed 6.1 / 12.3). Large tensors only without clusters (100 x 640 x 32 x 32
-  // 70.5 / 80, streamed 77.8 / 115; by clusters of four 48 x 320 x 64 x 64 82 / 92, streamed 72.6 / 94).
+  // block holds it (40 x 1280 x 16 x 16 by 80 bytes 24.9 us with three modules in flight / 28.7 alone, by 320 10.6 / 18.5, streamed 19.1 / 32.8). Few
+  // blocks per slab are best, for the sums of each cost the same: at most six where fewer hold it (2 x 320 x 96 x 96: by four 7.7 / 18.5, six
+  // 9.0 / 16.4, eight 11.3 / 22.6, streamed 10.4 / 20.5). Where a block leaves no room for a second one on its SM, nothing fills the time of its loads
+  // and sums: then only if they run at once, in clusters of up to six, on half of the SMs, else by more blocks (16 x 256 x 64 x 64 by two 17.8 /
+  // 22.6, by three 16.3 / 22.3, streamed 18.8 / 28.5; 6 x 62 x 100 x 100 by seven 6.2 / 16.4, streamed 5.9 / 12.3; 2 x 320 x 128 x 128 by seven 17.5 /
+  // 32.8, streamed 15.6 / 26.7). Large tensors only without clusters (100 x 640 x 32 x 32 70.5 / 80, streamed 70.5 / 97; by clusters of four
+  // 48 x 320 x 64 x 64 82 / 92, streamed 65 / 83). A block of 128 threads where they have two vectors or fewer each (3000 x 64 x 3 x 3 9.9 / 14.4,
+  // by 512 threads 35.6 / 39.0).
   int wide = (4 + unit_vecs - 1) / unit_vecs;
   while (2 * wide * unit_vecs <= kSlabThreads && (long long)n * ((units + 2 * wide - 1) / (2 * wide)) >= 2LL * sm_count &&
          (long long)pixels * 2 * wide * unit_vecs * 16 <= 90 * 1024)
@@ -203,9 +205,15 @@ inline GroupNormPlan group_norm_plan(int n, int pixels, int c, int groups, int e
     auto try_slab = [&](int parts) {
       if (parts > 8 || (large && parts > 1 && mode == 0)) return false;
       lay_out(kSlabThreads, wide, parts);
+      if (parts == 1 && p.vecs <= kSmallSlabThreads && pixels * p.vecs <= 2 * kSmallSlabThreads) {
+        lay_out(kSmallSlabThreads, wide, 1);
+        p.smem += (size_t)p.chunk_groups * 16 + (size_t)p.nv * kSmallSlabThreads * 16;
+        p.form = NORM_SLAB;
+        return true;
+      }
       p.smem = fixed + (size_t)p.nv * kSlabThreads * 16;
       p.form = NORM_SLAB;
-      return p.smem <= half || (slabs * p.parts <= sm_count && 2 * slabs * p.parts >= sm_count);
+      return p.smem <= half || (p.parts <= 6 && slabs * p.parts <= sm_count && 2 * slabs * p.parts >= sm_count);
     };
     const int need = parts_in(2 * half);
     const long long spread = std::min({6LL, sm_count / slabs, (pixels + 2 * lanes - 1) / (2 * lanes)});
