@@ -100,7 +100,8 @@ template <int ACT, bool F32> __device__ __forceinline__ Pair activate(Pair v) {
   if (ACT == ACT_GELU_TANH) return over_one_plus_exp2(v, v * fma(v * v, both(-0.10294324f), both(-2.3022082f)));
   return v;
 }
-// `use` is called with the activation as a compile-time constant
+// `use` is called with the activation as a compile-time constant, in a kernel or on the host
+#pragma nv_exec_check_disable
 template <class Use> __host__ __device__ inline void with_activation(int act, Use use) {
   switch (act) {
   case ACT_RELU: use(std::integral_constant<int, ACT_RELU>()); break;
