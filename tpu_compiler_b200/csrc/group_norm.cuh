@@ -114,7 +114,8 @@ __device__ __forceinline__ float block_sum(float v, float *red) {
 
 // ---- rows: groups of one pixel. LANES: 8 or 32 lanes of a warp per R groups, 0: a block. NV: vectors per thread. FULL: every thread has that
 // many, of channels only; the threads' means and squares are then joined in one exchange instead of two.
-// gamma and beta are four times the bytes of a BF16 vector: with one row at a time the L1's data path was 61% busy (4099 x 4096: 15.0 us).
+// gamma and beta are four times the bytes of a BF16 vector: with one row at a time the L1's data path was 61% busy (4099 x 4096: 15.0 us with
+// three modules in flight, with two 13.9, 4.8 TB/s: bound by memory, with one set of loads per block to hide it).
 template <typename T, int NV, int R, int LANES, bool FULL> __global__ void __launch_bounds__(LANES ? 128 : 512) group_norm_rows_kernel(const GroupNormArgs a) {
   typedef NormVec<T> V;
   constexpr bool BLOCK = LANES == 0;
