@@ -69,8 +69,8 @@ int tpucb_interp_set_weight(tpucb_interp *it, const char *name, const float *dat
  * y = act(x filter^T + bias) + residual: a fully_connected line that names an activation or an operand 7 (a tensor of y's shape and type).
  * do_relu=1 beside a residual is activation=relu; both attributes at once are refused, and so are filters of rank 3. gelu is
  * x Phi(x), gelu_tanh its approximation by tanh; silu, gelu and gelu_tanh go to zero for large negative values and are NaN (infinity times zero) for
- * minus infinity, as their definitions are in floating-point arithmetic. BF16 results of these two are rounded to nearest even, infinities and NaN kept, sums,
- * statistics and activations are fp32; a NaN or an infinity stays within its group or row. The order of sums depends on the shapes,
+ * minus infinity, as their definitions are in floating-point arithmetic. BF16 results of these two, and the filter of the second, are rounded to nearest even, infinities
+ * and NaN kept; sums, statistics and activations are fp32; a NaN or an infinity stays within its group or row. The order of sums depends on the shapes,
  * the options and the GPU's number of SMs alone: a module gives the same bits every time. */
 int tpucb_interp_load_module(tpucb_interp *it, const char *module_text);
 

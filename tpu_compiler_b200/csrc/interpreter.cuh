@@ -1905,7 +1905,7 @@ public:
       }
       return (const void *)I.upload(w);
     };
-    const void *w = out->dtype == DT_F32 ? packed(0.0f, [](float v) { return v; }) : packed((uint16_t)0, [](float v) { return f32_to_bf16_bits(v); });
+    const void *w = out->dtype == DT_F32 ? packed(0.0f, [](float v) { return v; }) : packed((uint16_t)0, [](float v) { return bf16_bits_ieee(v); });
     if (out->dtype == DT_F32) {
       f32_plan_ = linear_f32_plan(s.m, s.k_dev, out->cp, I.sm_count, I.linear_tiles);
       f32_ = LinearF32Args{(const float *)in->dev, (const float *)w, res_ ? (const float *)res_->dev : nullptr, bias, (float *)out->dev,

@@ -4,6 +4,7 @@
 #include "module_text.h"
 
 #include <cmath>
+#include <cstring>
 #include <functional>
 
 namespace tpucb {
@@ -53,6 +54,15 @@ inline GroupNormSpec group_norm_spec(const ParsedOp &op, const DevTensor &in, co
   s.gamma = affine(1, 1.0f);
   s.beta = affine(2, 0.0f);
   return s;
+}
+
+// The BF16 value that IEEE 754 rounds an fp32 one to (nearest even, infinities and NaN kept, overflow to infinity): weights of products whose
+// results are rounded that way. (f32_to_bf16_bits makes the largest finite value of all that is not finite, whatever its sign.)
+inline uint16_t bf16_bits_ieee(float v) {
+  uint32_t u;
+  std::memcpy(&u, &v, 4);
+  if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)(u >> 16 | 0x40u);
+  return (uint16_t)((u + 0x7fffu + (u >> 16 & 1u)) >> 16);
 }
 
 // fully_connected whose line names an activation or, as operand 7 behind the quantisation operands, a residual tensor.
