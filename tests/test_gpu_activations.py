@@ -6,10 +6,10 @@ Tolerances, relative to the value. u = 2^-24; h, the rounding of the result: 2^-
 gives 2^-22 = 4 u for ex2.approx and one unit in the last place, 2 u, for rcp.approx.
 * v / (1 + 2^t) by one reciprocal for two values: 4 u, 2 u, and five roundings (the sum, the product of two denominators, its share of the
   reciprocal, v times it, and the residual's sum): 11 u; t itself is off by its constants and products, 2 u |t| (SiLU) or 4 u |t| (tanh GELU), which
-  ln 2 carries into 2^t. From t = 60 on the value may count as zero: what is lost is below 2^-60 |v|.
+  ln 2 carries into 2^t. fp32: from t = 60 on the value may count as zero: what is lost is below 2^-60 |v|. BF16: 2^-61 is taken from the quotient.
 * |v| Q(|v|) = |v| 2^x P(t), x = -v^2 / 2 log2 e: 4 u of the exponential, 3 u |x| ln 2 = 1.5 u v^2 of its argument, 5 u of t = 1 / (1 + 0.35 |v|), which
   are 12 u of P (|t P' / P| < 2.3 up to |v| = 14), 16 u of P's eight steps (its terms add up to less than 1.9 times its value), two products, and P's
-  fit, 3.1e-7 (fp32) or 2.4e-5 (BF16): 38 u with some room. Positive v: max(v, 0) minus that, one rounding more.
+  fit, 3.1e-7 (fp32) or 2.4e-5 (BF16): 38 u with some room. Positive v: max(v, 0) minus that in one multiply-add.
 Below 2^-126 the exponential is flushed to zero.
 """
 from math import erfc, log, pi, sqrt
@@ -49,7 +49,8 @@ def value_and_tolerance(v, act, dtype):
         else:
             t = -v / log(2.0) if act == "silu" else -2.0 * sqrt(2.0 / pi) * (v + 0.044715 * v ** 3) / log(2.0)
             y = v / (1.0 + np.exp2(t))
-            own = (11 + (2 if act == "silu" else 4) * log(2.0) * np.abs(t)) * U * np.abs(y) + np.where(t >= 59.9, 2.0 ** -59.9 * np.abs(v), 0.0)
+            own = (11 + (2 if act == "silu" else 4) * log(2.0) * np.abs(t)) * U * np.abs(y)
+            own = own + (2.0 ** -61 if dtype == "BF16" else np.where(t >= 59.9, 2.0 ** -59.9, 0.0)) * np.abs(v)
         y = np.where(np.isnan(v), np.nan, y)
         return y, np.where(np.isfinite(y), own + h * np.abs(y), 0.0)
 

@@ -59,56 +59,54 @@ __device__ __forceinline__ Pair reciprocals(Pair a) {
   const float r = rcp_approx(a.lo() * a.hi());
   return Pair(a.hi() * r, a.lo() * r);
 }
-// v / (1 + 2^t). The exponent is held at 60, so that the product of two denominators stays in range; from 61 on the quotient counts as zero (between
-// them it is scaled down), which takes less than 2^-60 |v| from it: 3.6e-17 for SiLU, whose t passes 60 at v = -41.6, and 6.5e-18 for tanh GELU, at
-// -7.5. (With the quotient left at 2^-60 SiLU of -1e20 was -87.) Minus infinity times that zero is a NaN, as it is where the definition is computed.
-// The zero costs 1 x 256 x 512 x 512 with SiLU 1.6% (70.2 -> 71.3 us with three modules in flight) and the slab's 8 x 320 x 64 x 64 nothing (12.8);
-// as a compare and a select per value instead of a saturated difference and a packed product 2% of both.
-__device__ __forceinline__ Pair over_one_plus_exp2(Pair v, Pair t) {
-  const Pair there(__saturatef(61.0f - t.lo()), __saturatef(61.0f - t.hi()));
-  return v * there * reciprocals(Pair(ex2_approx(fminf(t.lo(), 60.0f)), ex2_approx(fminf(t.hi(), 60.0f))) + both(1.0f));
-}
-__device__ __forceinline__ float max_or_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
+// v / (1 + 2^t). The exponent is held at 62, so that the product of two denominators stays in range, and for large t the quotient goes to zero itself,
+// because v may be large (left at its last value SiLU of -1e20 was -87). Minus infinity times that zero is a NaN, as where the definition is computed.
+//   fp32: a factor that falls from 1 at t = 60 to 0 at t = 61: what is lost is below 2^-60 |v|.
+//   BF16: 2^-61 is taken from the quotient in the multiply-add that forms it, which saturates at zero. Up to t = 52, SiLU of -36, that is less than
+//   half a step of the result; in all it is below 2^-61 |v|. (The factor's three instructions: 64 x 256 x 32 x 32 with SiLU 14.7 -> 15.3 us with three
+//   modules in flight, these none.)
+template <bool F32> __device__ __forceinline__ Pair over_one_plus_exp2(Pair v, Pair t) {
+  const Pair d = Pair(ex2_approx(fminf(t.lo(), 62.0f)), ex2_approx(fminf(t.hi(), 62.0f))) + both(1.0f);
+  if (F32) return v * Pair(__saturatef(61.0f - t.lo()), __saturatef(61.0f - t.hi())) * reciprocals(d);
+  const float r = rcp_approx(d.lo() * d.hi());
+  return v * Pair(__saturatef(fmaf(d.hi(), r, -4.3368087e-19f)), __saturatef(fmaf(d.lo(), r, -4.3368087e-19f)));
 }
 
 // gelu(v) = v Phi(v) = max(v, 0) - |v| Q(|v|), with the upper tail of the normal distribution Q(a) = erfc(a / sqrt 2) / 2 =
 // e^(-a^2/2) P(1 / (1 + p a)): no cancellation on either side. The polynomials P are this file's own minimax fits of
 // e^(a^2/2) Q(a) over a in [0, 14] (beyond, Q is below 1e-44): largest relative error 2.4e-5 for BF16 results, a hundredth of
 // their rounding, and 3.1e-7 for fp32 ones. The exponent's rounding adds up to 1.5 2^-24 a^2 of the tail: in all 8e-7 of the value
-// down to -3, 1.3e-6 to -5 (a value of 1.4e-6), 7.6e-6 to -12 (2e-32), measured. (Beyond 2^40 the reciprocals of a pair would leave the range: a is held there, but not as a factor, so that minus infinity
-// gives infinity times zero, a NaN.)
+// down to -3, 1.3e-6 to -5 (a value of 1.4e-6), 7.6e-6 to -12 (2e-32), measured. (Beyond 2^40 the reciprocals
+// of a pair would leave the range: a is held there.) v / 2 + |v| / 2 is max(v, 0), and for minus infinity a NaN, as where the definition is computed.
 template <bool F32> __device__ __forceinline__ Pair gelu_exact(Pair v) {
   const Pair a(fminf(fabsf(v.lo()), 1.0995116e12f), fminf(fabsf(v.hi()), 1.0995116e12f));
   const Pair t = reciprocals(fma(both(0.35f), a, both(1.0f))), x = a * a * both(-0.7213475204444817f);
   const Pair e(ex2_approx(x.lo()), ex2_approx(x.hi()));
-  Pair q;
+  Pair q; // -P
   if (F32) {
-    q = fma(both(0.04894244623667017f), t, both(-0.2021192868271973f));
-    q = fma(q, t, both(0.24064081895892164f));
-    q = fma(q, t, both(-0.01702343620260618f));
-    q = fma(q, t, both(0.15596148733152987f));
-    q = fma(q, t, both(0.13335509625098455f));
-    q = fma(q, t, both(0.14027034361266144f));
-    q = fma(q, t, both(-2.731554772757582e-05f));
+    q = fma(both(-0.04894244623667017f), t, both(0.2021192868271973f));
+    q = fma(q, t, both(-0.24064081895892164f));
+    q = fma(q, t, both(0.01702343620260618f));
+    q = fma(q, t, both(-0.15596148733152987f));
+    q = fma(q, t, both(-0.13335509625098455f));
+    q = fma(q, t, both(-0.14027034361266144f));
+    q = fma(q, t, both(2.731554772757582e-05f));
   } else {
-    q = fma(both(-0.09778110211354195f), t, both(0.278881467362648f));
-    q = fma(q, t, both(0.010946683641198824f));
-    q = fma(q, t, both(0.17298857188677733f));
-    q = fma(q, t, both(0.13469103084119843f));
-    q = fma(q, t, both(0.0002850549969567228f));
+    q = fma(both(0.09778110211354195f), t, both(-0.278881467362648f));
+    q = fma(q, t, both(-0.010946683641198824f));
+    q = fma(q, t, both(-0.17298857188677733f));
+    q = fma(q, t, both(-0.13469103084119843f));
+    q = fma(q, t, both(-0.0002850549969567228f));
   }
-  // min(v, -a) is -|v|, and minus infinity where v is
-  return fma(Pair(fminf(v.lo(), -a.lo()), fminf(v.hi(), -a.hi())), q * e, Pair(max_or_nan(v.lo(), 0.0f), max_or_nan(v.hi(), 0.0f)));
+  const Pair h = v * both(0.5f);
+  return fma(a, q * e, Pair(h.lo() + fabsf(h.lo()), h.hi() + fabsf(h.hi())));
 }
 template <int ACT, bool F32> __device__ __forceinline__ Pair activate(Pair v) {
   if (ACT == ACT_RELU) return Pair(v.lo() < 0.0f ? 0.0f : v.lo(), v.hi() < 0.0f ? 0.0f : v.hi());
-  if (ACT == ACT_SILU) return over_one_plus_exp2(v, v * both(-1.4426950408889634f));
+  if (ACT == ACT_SILU) return over_one_plus_exp2<F32>(v, v * both(-1.4426950408889634f));
   if (ACT == ACT_GELU) return gelu_exact<F32>(v);
   // 0.5 v (1 + tanh u) = v / (1 + e^(-2u)), u = sqrt(2 / pi) (v + 0.044715 v^3)
-  if (ACT == ACT_GELU_TANH) return over_one_plus_exp2(v, v * fma(v * v, both(-0.10294324f), both(-2.3022082f)));
+  if (ACT == ACT_GELU_TANH) return over_one_plus_exp2<F32>(v, v * fma(v * v, both(-0.10294324f), both(-2.3022082f)));
   return v;
 }
 // `use` is called with the activation as a compile-time constant, in a kernel or on the host
