@@ -10,13 +10,17 @@
 //            exchange their statistics through it: x is read once;
 //   streamed larger ones: a pass for the statistics of parts of an image, and a pass that joins them and forms the results, in the
 //            opposite order, so that it begins with what the L2 still holds;
-//   strided  groups of more than 512 vectors, if not one pixel's: the same two passes, value by value.
-// Variances are never differences of large sums. Rows and slab take the mean first and then the squares of the distances from it, out
-// of the registers (slab: from the mean of the block). Streamed sums distances from the first value that a thread sees in a channel, and
-// their squares: the error is then at most the thread's count times 2^-24 of the variance, even where that value is an outlier (it is part
-// of the variance; one such value for the whole block cost 1e-4 of it). Partial ones are joined as
+//   strided  the same two passes, value by value: images where the smallest run of whole groups that is also whole vectors has more than 256
+//            vectors and does not fit a slab, or more than 512 (2 x 2560 x 32 x 32 in one group: 320 vectors).
+// Rows take the mean first and then the squares of the distances from it, out of the registers. The other forms sum, in one pass, the distances
+// from the first value that a thread sees (in a channel, or in all of its vectors where they lie within a group) and their squares, and take
+// q - s s / n: a difference, whose error is at most 2 (L + 4) (L + 1) 2^-24 of the variance for the L values that a thread sums one after the other, also
+// where the first value is an outlier, which is part of the variance itself. (One such value for the whole block cost 1e-4 of it.) Partial ones are joined
+// without differences of sums:
 //   M2 = sum M2_i + sum n_i (mean_i - mean)^2.
-// The result is one multiply-add per value, with beta - mean rstd gamma rounded once, an error like that of the mean itself.
+// The result is one multiply-add per value, with beta - mean rstd gamma rounded once. Its error is like that of the mean itself, a few 2^-24 |mean| rstd
+// gamma: in a group of equal values c, whose rstd is 1 / sqrt(eps), beta is met to that (c = 10, eps = 1e-5: 6e-5), as in a plain fp32
+// form whose mean is rounded.
 #pragma once
 #include "activation.cuh"
 #include "conv_plan.cuh"
@@ -428,8 +432,8 @@ template <typename T> struct NormAffine {
 
 // ---- slab. ALIGNED: a vector's channels belong to one group. A thread's vectors wait in shared memory, [vector][thread], where it alone writes
 // and reads them: no barrier orders them. Bound by the memory's latency and the sums between its two halves, which other blocks of the SM fill where
-// there are any: 64 x 256 x 32 x 32 with SiLU 14.2 us with three modules in flight (72% of the memory's rate), 8 x 320 x 64 x 64 12.8, alone
-// 18.5. (With the vectors in registers, eight per thread, those took 22.8, 25.1 and 28.7 us: a wave of blocks held half as much, in one block
+// there are any: 64 x 256 x 32 x 32 with SiLU 14.8 us with three modules in flight (69% of the memory's rate), 8 x 320 x 64 x 64 12.8, one
+// module's launches behind one another 18.5. (With the vectors in registers, eight per thread, those took 22.8, 25.1 and 28.7 us: a wave of blocks held half as much, in one block
 // per SM.)
 template <typename T, bool ALIGNED, int THREADS> __global__ void __launch_bounds__(THREADS, 1024 / THREADS) group_norm_slab_kernel(const GroupNormArgs a) {
   extern __shared__ __align__(16) float smem[];
@@ -631,7 +635,8 @@ template <typename T, bool ALIGNED> __global__ void __launch_bounds__(kStreamThr
 }
 
 // ---- strided: groups of any width, value by value, a block per part of a group; statistics and results as in the streamed form. Bound by its
-// instructions: 2 x 2560 x 32 x 32 with one group 26.7 us (one block per group 5525).
+// instructions: 2 x 2560 x 32 x 32 with one group 16.3 us with three modules in flight (20% of the memory's rate), one module's launches behind one
+// another 27.6 (one block per group 5525).
 template <typename T, class Use> __device__ __forceinline__ void for_group_values(const GroupNormArgs &a, Use use) { // use(offset, channel)
   const unsigned lot = blockIdx.x / a.parts, part = blockIdx.x - lot * a.parts, img = lot / a.groups, g = lot - img * a.groups;
   const long long from = part * a.part_values, to = min(from + a.part_values, (long long)a.pixels * a.cg);

@@ -2720,7 +2720,7 @@ inline void Interpreter::sync_and_check() {
     *ss.h_err = 0;
     TPUCB_CUDA(cudaMemsetAsync(&ss.d_err->code, 0, sizeof(int), stream));
     for (auto &w : split_ws) TPUCB_CUDA(cudaMemsetAsync(w.first, 0, w.second, stream)); // a failed launch may leave partial sums
-    throw Error(strfmt("a convolution kernel gave up on a bounded wait (code %d: 1 = tile load never arrived, "
+    throw Error(strfmt("a tensor-core kernel gave up on a bounded wait (code %d: 1 = tile load never arrived, "
                        "2 = stage never freed, 3 = accumulator never completed or never handed back); the launch's "
                        "results are incomplete, the interpreter stays usable", err));
   }

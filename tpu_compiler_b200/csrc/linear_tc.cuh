@@ -9,13 +9,14 @@
 //   (128 + nt / 2) x 128 bytes of copies. Accumulators are double-buffered: the epilogue of a tile runs beside the next one's loop; its
 //   warps write 32 rows x 32 channels through shared memory by bulk tensor stores, clipped by their map (sectors stored by the threads:
 //   8192 x 256 x 8192 59 us, now 47). Bound by the tensor pipe, and with work in flight all the time by the power limit: 8192 x 4096 x 4096
-//   with a residual 176 us in a single launch (1.56 PFLOP/s, pipe 92% active), 210 to 229 with three modules in flight.
+//   with a residual 176 us in a single launch (1.56 PFLOP/s, pipe 92% active), 210 to 229 with three modules in flight. The accumulators cut
+//   what an fp32 multiply-add rounds: about 1e-5 of a value at K = 4096, which moves one BF16 result in 400 to its neighbour.
 // linear_split_kernel, for the others, down to one row: tiles of 128 rows x nt channels, and a cluster of up to eight CTAs that
 //   share a tile's K, so that few rows still draw weights through all SMs. The partial sums meet in shared memory: every CTA adds up
 //   its share of the columns from all of the cluster, in the order of K (no atomics, the same bits every time), and finishes it.
 //   Copies of x take as many rows as there are; the tensor memory is given back before a CTA waits for the others of its
 //   cluster (two clusters on the same SMs could otherwise wait for each other's). Bound by memory where K and the channels are long
-//   (1 x 4096 x 4096 6.1 us with three modules in flight, 84% of the copy rate; 1 x 8192 x 8192 19.9), by latency below.
+//   (1 x 4096 x 4096 with a residual 6.6 us with three modules in flight, 78% of the copy rate; 1 x 8192 x 8192 19.9), by latency below.
 // Weights are fetched before the previous kernel's results are waited for (programmatic dependent launch). Every wait is bounded as in
 // conv_gemm_i8.cuh.
 #pragma once

@@ -123,7 +123,8 @@ struct GroupNormPlan {
   long long part_values = 0; // strided: of a group, per block
   size_t smem = 0;
 };
-// mode (option "norm_form"): 0 by size, else 1 + the form, where it can
+// mode (option "norm_form"): 0 by size, else 1 + the form, where it can.
+// Times in the comments are us per launch with three modules in flight / with one module's launches behind one another ("in a row").
 inline GroupNormPlan group_norm_plan(int n, int pixels, int c, int groups, int es, int sm_count, int mode) {
   const int N = 16 / es, cg = c / groups;
   GroupNormPlan p;
@@ -192,7 +193,7 @@ inline GroupNormPlan group_norm_plan(int n, int pixels, int c, int groups, int e
   // Tensors whose passes take long enough that only their loops count: from 128 vectors per thread of the streamed form on.
   const bool large = (long long)n * pixels * ((c + N - 1) / N) >= 128LL * kStreamThreads * sm_count;
   // slab: 64 bytes of a pixel and more, in the shared memory of at most eight blocks; more of a pixel while two blocks per SM remain and one
-  // block holds it (40 x 1280 x 16 x 16 by 80 bytes 24.9 us with three modules in flight / 28.7 alone, by 320 10.6 / 18.5, streamed 19.1 / 32.8). Few
+  // block holds it (40 x 1280 x 16 x 16 by 80 bytes 24.9 / 28.7, by 320 10.6 / 18.5, streamed 19.1 / 32.8). Few
   // blocks per slab are best, for the sums of each cost the same: at most six where fewer hold it (2 x 320 x 96 x 96: by four 7.7 / 18.5, six
   // 9.0 / 16.4, eight 11.3 / 22.6, streamed 10.4 / 20.5). Where a block leaves no room for a second one on its SM, nothing fills the time of its loads
   // and sums: then only if they run at once, in clusters of up to six, on half of the SMs, else by more blocks (16 x 256 x 64 x 64 by two 17.8 /
@@ -235,7 +236,7 @@ inline GroupNormPlan group_norm_plan(int n, int pixels, int c, int groups, int e
   lay_out(kStreamThreads, most_units, 1);
   const long long slabs = (long long)n * p.chunks, per_part = 8LL * p.lanes;
   auto parts_of = [&](int blocks) { return (int)std::max(1LL, std::min((long long)blocks * sm_count / slabs, (pixels + per_part - 1) / per_part)); };
-  // Blocks per SM of the two passes. Few leave fewer partial statistics and less around the loops, many hide the memory's latency; us alone /
+  // Blocks per SM of the two passes. Few leave fewer partial statistics and less around the loops, many hide the memory's latency; us in a row /
   // with three modules in flight, (1, 1), (1, 2), (2, 3): 4 x 128 x 128 x 128 24.6 / 10.7, 22.5 / 12.0, 20.5 / 13.8; 8 x 320 x 64 x 64
   // 28.7 / 14.1, 26.6 / 15.2, 22.6 / 16.5; 1 x 256 x 512 x 512 106 / 65, 91 / 71, 85 / 66; fp32 2 x 100 x 400 x 400 129 / 83, 116 / 83, 90 / 70.
   const int fs = large ? 2 : 1, fa = large ? 3 : 2;
@@ -289,7 +290,7 @@ inline LinearTcPlan linear_tc_sizes(bool pair, int nt, int split, int m, int k_d
   return l;
 }
 // mode (option "linear_tiles"): 1 by size; 1000 * split + nt; 10000 + nt: pairs
-// By size; us with three modules in flight / alone:
+// By size; us with three modules in flight / in a row:
 //   Pairs where there are more tiles of 128 x 64 than SMs, and more than one of rows; 256 channels, 128 where those leave half of the
 //   pairs idle. 256 x 4096 x 16384 31 / 37 (clusters of one 35 / 62), 8192 x 4096 x 4096 190 / 180 (222 / 240), 600 x 1000 x 5000 8.8 / 14.4 (8.8 /
 //   18.3), 2048 x 512 x 2048 7.1 / 10.3 (6.7 / 12.3); 512 x 4096 x 4096 with 256 channels 14.0 / 26.8, with 128 15.6 / 18.6.
